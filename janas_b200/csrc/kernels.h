@@ -158,6 +158,20 @@ int jb_norm_residual(float *x, const float *a, int Sa, long long a_stride, const
                      const void *skip, int skip_dt, const float *coef, int coef_ld, const float *w,
                      const float *bias, int n, int dm, float eps, int rms, int few_rows,
                      cudaStream_t st);
+int jb_norm_residual_norm(float *x, const float *y, int Sy, long long y_stride, const float *y_bias,
+                          const float *g, int Sg, long long g_stride, int g_ld, int g_col0, const float *g_bias,
+                          const float *w1, const float *b1, float eps1, const float *scale, float mult,
+                          const float *w2, const float *b2, float eps2, int rms, void *out, void *out_scales,
+                          int out_kind, int n, int dm, cudaStream_t st);
+int jb_norm_residual_norm_most(void);
+long long jb_mx4_code_bytes(int rows, int k);
+long long jb_mx4_scale_bytes(int rows, int k);
+int jb_mx4_quantize(const void *x, int dt, void *codes, void *scales, int n, int k, int early, cudaStream_t st);
+int jb_mx4_gated_unit(const float *z, int S, long long stride, void *codes, void *scales, int n, int ff,
+                      float alpha, float limit, float shift, cudaStream_t st);
+int jb_mx4_values(const void *codes, const void *scales, void *out, int out_dt, int n, int k, cudaStream_t st);
+int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales, void *out,
+                  int out_dt, int n, int m, int k, cudaStream_t st);
 int jb_short_conv(const float *x, const float *w, float *state, long long slot_stride, const int32_t *row_pos,
                   const int32_t *row_seq, const int32_t *seq_slot, void *out, int out_dt, int n,
                   int dm, int taps, int what, cudaStream_t st);

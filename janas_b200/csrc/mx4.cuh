@@ -1,0 +1,127 @@
+// Microscaled 4-bit floats: a block of 32 values along a row stands for 2^s times 32 numbers of one sign, two
+// exponent and one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6).
+//
+//   s = max(floor(log2 max |x|) - 2, -127),   number = x / 2^s rounded to nearest, ties to even, at most 6
+//
+// so the block's largest value lies in [4, 8) before the rounding and what lies above 6 becomes 6.  A block with a NaN
+// or an infinity stands for NaNs.  The last block of a row is filled up with zeros.
+//
+// In memory: codes [rows, 16 ceil(k / 32)] bytes, value 2i in the low half of byte i; scales [ceil(rows / 128),
+// ceil(k / 256), 1024] bytes, s + 127 (255: NaN), a chunk of 256 values of 128 rows together: in the order in which the
+// tensor cores take them (four consecutive blocks of row r at 16 (r % 32) + 4 (r / 32 % 4), the other four 512 behind).
+#pragma once
+
+#include "common.cuh"
+
+namespace jb {
+
+constexpr int MX4_CHUNK = 256;              // values of a row that a chunk of scales is for
+constexpr int MX4_TILE = 1024;              // its bytes, for 128 rows
+
+__host__ __device__ inline size_t mx4_row_bytes(int k) { return (size_t)((k + 31) / 32) * 16; }
+__host__ __device__ inline int mx4_chunks(int k) { return (k + MX4_CHUNK - 1) / MX4_CHUNK; }
+// the place of the first four (half 0) or last four (half 1) scales of row r's chunk c
+__host__ __device__ inline size_t mx4_scale_at(size_t r, int c, int chunks, int half)
+{
+    return ((r >> 7) * (size_t)chunks + (size_t)c) * MX4_TILE + half * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4;
+}
+
+// s + 127 of a block from the bits of its largest magnitude
+__device__ __forceinline__ uint32_t mx4_scale_code(uint32_t top)
+{
+    if (top >= 0x7f800000u)
+        return 255u;
+    uint32_t e = top >> 23;
+    return e > 2u ? e - 2u : 0u;
+}
+
+// 2^-s of a scale's code (0 .. 252); the products with it are exact
+__device__ __forceinline__ float mx4_inverse(uint32_t code)
+{
+    return __uint_as_float((254u - min(code, 252u)) << 23);
+}
+
+// 2^s (a subnormal float for the code 0, NaN for 255)
+__device__ __forceinline__ float mx4_scale(uint32_t code)
+{
+    return __uint_as_float(code == 255u ? 0x7fffffffu : code == 0u ? 0x00400000u : code << 23);
+}
+
+// Eight values times inv, rounded to 4 bits: value i in bits 4 i.
+__device__ __forceinline__ uint32_t mx4_pack8(const float *v, float inv)
+{
+    uint32_t r;
+    asm("{\n\t"
+        ".reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t"
+        "}\n"
+        : "=r"(r)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
+          "f"(v[6] * inv), "f"(v[7] * inv));
+    return r;
+}
+
+// The bits of the largest magnitude among eight values (a NaN is larger than an infinity).
+__device__ __forceinline__ uint32_t mx4_top8(const float *v)
+{
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
+    return t;
+}
+
+// A warp packs a row's chunk of 256 values, eight to a lane (zeros past the row's end): codes and scales to memory.
+__device__ __forceinline__ void mx4_store_chunk(const float *v, size_t r, int c, int k, uint8_t *__restrict__ codes,
+                                                uint8_t *__restrict__ scales)
+{
+    const int lane = threadIdx.x & 31;
+    uint32_t top = mx4_top8(v);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    uint32_t code = mx4_scale_code(top);
+    uint32_t packed = mx4_pack8(v, mx4_inverse(code));
+    const size_t row_bytes = mx4_row_bytes(k), at = (size_t)c * (MX4_CHUNK / 2) + lane * 4;
+    if (at < row_bytes)
+        *reinterpret_cast<uint32_t *>(codes + r * row_bytes + at) = packed;
+    // the codes of four blocks in one word: lanes 0, 4, 8, 12 of this half of the warp
+    uint32_t word = code;
+    word |= __shfl_down_sync(0xffffffffu, code, 4) << 8;
+    word |= __shfl_down_sync(0xffffffffu, code, 8) << 16;
+    word |= __shfl_down_sync(0xffffffffu, code, 12) << 24;
+    if ((lane & 15) == 0)
+        *reinterpret_cast<uint32_t *>(scales + mx4_scale_at(r, c, mx4_chunks(k), lane >> 4)) = word;
+}
+
+// The numbers that the 8 codes of a word stand for.
+__device__ __forceinline__ void mx4_unpack8(uint32_t word, float *v)
+{
+    uint32_t h[4];
+    asm("{\n\t"
+        ".reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t"
+        "}\n"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(word));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        asm("{\n\t"
+            ".reg .b16 lo, hi;\n\t"
+            "mov.b32 {lo, hi}, %2;\n\t"
+            "cvt.f32.f16 %0, lo;\n\t"
+            "cvt.f32.f16 %1, hi;\n\t"
+            "}\n"
+            : "=f"(v[2 * i]), "=f"(v[2 * i + 1])
+            : "r"(h[i]));
+    }
+}
+
+}  // namespace jb

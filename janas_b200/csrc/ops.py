@@ -465,6 +465,72 @@ def norm_residual_(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, eps: 
     return x
 
 
+def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[torch.Tensor],
+                       next_weight: Optional[torch.Tensor], eps: float, rms: bool = True,
+                       y_bias: Optional[torch.Tensor] = None, y_gate: Optional[torch.Tensor] = None, gate_col0: int = 0,
+                       gate_bias: Optional[torch.Tensor] = None, scale=None, post_bias: Optional[torch.Tensor] = None,
+                       next_bias: Optional[torch.Tensor] = None, out="float32", next_eps: Optional[float] = None):
+    """The end of a sublayer and the start of the next in one pass over the rows:
+
+        u = (sum y + y_bias) * sigmoid(sum g + gate_bias);   x += scale * N1(u), in place;   h = N2(x)
+
+    y and y_gate: stacks of partial sums; the gate is columns gate_col0 .. gate_col0 + dm - 1 of y_gate, None: no
+    gate.  scale: a float32 vector [dm] or a number, None: 1.  N1, N2: RMS norms, or with rms False layer norms, with
+    a weight and optionally a bias (float32 [dm]); post_weight None: N1(u) = u; next_weight None: no h, None is
+    returned.  h is [n, dm] in ``out``: torch.float32, torch.bfloat16, or "mx4" for an Mx4."""
+    _need(x, "x", torch.float32, (None, None))
+    _here(x, "x")
+    n, dm = x.shape
+    y = stack(y)
+    _need(y, "y", torch.float32, (None, n, dm))
+    at = x.device
+    for t, name in ((y_bias, "y_bias"), (gate_bias, "gate_bias"), (post_weight, "post_weight"), (post_bias, "post_bias"),
+                    (next_weight, "next_weight"), (next_bias, "next_bias")):
+        if t is not None:
+            _need(t, name, torch.float32, (dm,))
+            if t.device != at:
+                raise KernelError(f"{name}: on another device than x")
+    Sg, g_ld = 0, 0
+    if y_gate is not None:
+        y_gate = stack(y_gate)
+        _need(y_gate, "y_gate", torch.float32, (None, n, None))
+        Sg, _, g_ld = y_gate.shape
+        if Sg < 1 or gate_col0 < 0 or g_ld - gate_col0 < dm or y_gate.device != at:
+            raise KernelError("norm_residual_norm: the gate's columns lie outside y_gate, or it is on another device")
+    elif gate_bias is not None:
+        raise KernelError("norm_residual_norm: a gate_bias without a gate")
+    if (post_bias is not None and post_weight is None) or (next_bias is not None and next_weight is None):
+        raise KernelError("norm_residual_norm: a norm's bias without its weight")
+    if not y.shape[0] or y.device != at:
+        raise KernelError("norm_residual_norm: y needs at least one sum, on x's device")
+    mult = 1.0
+    if isinstance(scale, torch.Tensor):
+        _need(scale, "scale", torch.float32, (dm,))
+        if scale.device != at:
+            raise KernelError("scale: on another device than x")
+    elif scale is not None:
+        mult, scale = float(scale), None
+    h = codes = scales = None
+    kind = 0
+    if out == "float32":
+        out = torch.float32
+    if out != "mx4" and out not in _FLOATS:
+        raise KernelError(f"norm_residual_norm: h is float32, bfloat16 or \"mx4\", not {out}")
+    if next_weight is not None:
+        if out == "mx4":
+            h = Mx4._new(n, dm, at, False)
+            codes, scales, kind = h.codes, h.scales, 4
+        else:
+            h = codes = torch.empty((n, dm), dtype=out, device=at)
+            kind = _DT[out]
+    _check(lib().jb_norm_residual_norm(
+        _p(x), _p(y), y.shape[0], n * dm, _p(y_bias), _p(y_gate), Sg, n * g_ld, g_ld, gate_col0, _p(gate_bias),
+        _p(post_weight), _p(post_bias), float(eps), _p(scale), mult, _p(next_weight), _p(next_bias),
+        float(eps if next_eps is None else next_eps), 1 if rms else 0, _p(codes), _p(scales), kind, n, dm, _stream()),
+        "norm_residual_norm", 1 if n else 0)
+    return h
+
+
 def short_conv(x: torch.Tensor, w: torch.Tensor, state: Optional[torch.Tensor], row_pos: torch.Tensor,
                row_seq: torch.Tensor, seq_slot: torch.Tensor, out_dtype: torch.dtype,
                write_h: bool = True, write_state: bool = True) -> Optional[torch.Tensor]:
@@ -1254,6 +1320,115 @@ def linear_swiglu(a: torch.Tensor, gate_up: torch.Tensor, alpha: float = 1.0, li
     _check(lib().jb_gemm_tc_gated(_p(a), _p(gate_up), _p(out), n, ff, k, float(alpha), float(limit),
                                   float(shift), _stream()),
            "linear_swiglu (tcgen05)")
+    return out
+
+
+class Mx4:
+    """A matrix [rows, k] in microscaled 4-bit floats, in device memory.
+
+    ``codes``: uint8 [rows, 16 ceil(k / 32)], value 2i of a row in the low half of byte i;
+    ``scales``: uint8 [ceil(rows / 128), ceil(k / 256), 1024], for each 128 rows and 256 of k the
+    exponents + 127 of the blocks of 32 values (255: the block stands for NaNs), block b of row r
+    at 512 (b / 4) + 16 (r % 32) + 4 (r / 32 % 4) + b % 4.  Bytes of rows past the last one are
+    not written and not used."""
+
+    __slots__ = ("codes", "scales", "rows", "k", "settled")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int):
+        if k < 1 or rows < 0:
+            raise KernelError("Mx4: rows of at least one value are needed")
+        _need(codes, "codes", torch.uint8, (rows, (k + 31) // 32 * 16))
+        _need(scales, "scales", torch.uint8, ((rows + 127) // 128, (k + 255) // 256, 1024))
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16 or codes.device != scales.device:
+            raise KernelError("Mx4: codes and scales must lie on one device at addresses that 16 divides")
+        self.codes, self.scales, self.rows, self.k = codes, scales, rows, k
+        # whether no kernel that may start before the writer's end can follow the writer
+        self.settled = True
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.rows, self.k)
+
+    @classmethod
+    def _new(cls, rows: int, k: int, device: torch.device, settled: bool) -> "Mx4":
+        if k < 1:
+            raise KernelError("Mx4: rows of at least one value are needed")
+        self = object.__new__(cls)
+        self.codes = torch.empty((rows, (k + 31) // 32 * 16), dtype=torch.uint8, device=device)
+        self.scales = torch.empty(((rows + 127) // 128, (k + 255) // 256, 1024), dtype=torch.uint8, device=device)
+        self.rows, self.k, self.settled = rows, k, settled
+        return self
+
+
+def _here(t: torch.Tensor, name: str) -> None:
+    """The launch goes to the current device's stream: a tensor of another device is refused."""
+    if t.get_device() != torch.cuda.current_device():
+        raise KernelError(f"{name}: on {t.device}, but the current device is {torch.cuda.current_device()}")
+
+
+def mx4_quantize(x: torch.Tensor) -> Mx4:
+    """x [n, k] (float32 or bfloat16) in microscaled 4-bit floats: each block of 32 values along a row
+    as 2^s times numbers of {0, 0.5, 1, 1.5, 2, 3, 4, 6} and a sign, s = floor(log2 max |x|) - 2 (at least
+    -127), rounded to nearest, ties to even, at most 6.  A block with a NaN or an infinity stands for NaNs."""
+    _need(x, "x", _FLOATS, (None, None))
+    _here(x, "x")
+    n, k = x.shape
+    q = Mx4._new(n, k, x.device, True)
+    _check(lib().jb_mx4_quantize(_p(x), _DT[x.dtype], _p(q.codes), _p(q.scales), n, k, 0, _stream()), "mx4_quantize",
+           1 if n else 0)
+    return q
+
+
+def mx4_gated_unit(gate_up: torch.Tensor, alpha: float = 1.0, limit: float = 0.0, shift: float = 0.0) -> Mx4:
+    """``swiglu`` of a stack [S, n, 2 ff] with the result in microscaled 4-bit floats, [n, ff]."""
+    gate_up = stack(gate_up)
+    _need(gate_up, "gate_up", torch.float32, (None, None, None))
+    _here(gate_up, "gate_up")
+    S, n, two_ff = gate_up.shape
+    if two_ff % 2 or not S:
+        raise KernelError("mx4_gated_unit: the gate_up width must be even, and at least one sum is needed")
+    q = Mx4._new(n, two_ff // 2, gate_up.device, False)
+    _check(lib().jb_mx4_gated_unit(_p(gate_up), S, n * two_ff, _p(q.codes), _p(q.scales), n, two_ff // 2, float(alpha),
+                                   float(limit), float(shift), _stream()), "mx4_gated_unit", 1 if n else 0)
+    return q
+
+
+def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """What q stands for, as [rows, k] in float32 or bfloat16 (both hold every value exactly)."""
+    _here(q.codes, "q")
+    if out_dtype not in _FLOATS:
+        raise KernelError(f"mx4_values: the output is float32 or bfloat16, not {out_dtype}")
+    out = torch.empty((q.rows, q.k), dtype=out_dtype, device=q.codes.device)
+    _check(lib().jb_mx4_values(_p(q.codes), _p(q.scales), _p(out), _DT[out_dtype], q.rows, q.k, _stream()), "mx4_values",
+           1 if q.rows else 0)
+    return out
+
+
+def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """a [n, k] . w [m, k]^T with both in microscaled 4-bit floats, summed in float32: [n, m] in float32 or
+    bfloat16, the result itself and no stack of parts.  ``a``: an Mx4, or float32 or bfloat16 rows, which are
+    brought to 4 bits first, as mx4_quantize does."""
+    if not isinstance(w, Mx4):
+        raise KernelError("linear_mx4: the weight is an Mx4 (see mx4_quantize)")
+    if out_dtype not in _FLOATS:
+        raise KernelError(f"linear_mx4: the output is float32 or bfloat16, not {out_dtype}")
+    if not isinstance(a, Mx4):
+        _need(a, "activations", _FLOATS, (None, w.k))
+        _here(a, "activations")
+        n = a.shape[0]
+        q = Mx4._new(n, w.k, a.device, False)
+        _check(lib().jb_mx4_quantize(_p(a), _DT[a.dtype], _p(q.codes), _p(q.scales), n, w.k, 1, _stream()),
+               "linear_mx4", 1 if n else 0)
+        a = q
+    elif a.k != w.k:
+        raise KernelError(f"linear_mx4: rows of {a.k} values and a weight of {w.k}")
+    else:
+        _here(a.codes, "activations")
+    _here(w.codes, "weight")
+    n, m = a.rows, w.rows
+    out = torch.empty((n, m), dtype=out_dtype, device=w.codes.device)
+    _check(lib().jb_linear_mx4(_p(a.codes), _p(a.scales), _p(w.codes), _p(w.scales), _p(out), _DT[out_dtype], n, m, w.k,
+                               _stream()), "linear_mx4", 1 if n and m else 0)
     return out
 
 
