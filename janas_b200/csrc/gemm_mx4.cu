@@ -1,75 +1,361 @@
-// Products of microscaled 4-bit floats (mx4.cuh):
+// Products of microscaled 4-bit floats (mx4.cuh) on the fifth-generation tensor cores:
 //
 //     out[r, f] = sum over blocks b of 2^(sa[r, b] + sw[f, b]) * sum over i in b of pa[r, i] pw[f, i]
 //
-// A thread per output.  Twice a 4-bit number is a whole number up to 12, so a block's sum is exact in integers; the
-// blocks' sums are added in float32, in order.
+// by block-scaled MMAs (kind::mxf4), which take both operands' codes from shared memory and both operands' scales from
+// tensor memory and add up in float32.  The weights are the M operand (128 features a tile), the rows the N operand.
+//
+// A CTA computes 128 features by BN rows over one part of k; the parts of a tile are the CTAs of a cluster, which add
+// their sums up in the order of k through distributed shared memory, so the result comes out whole.  Warp 0 loads
+// stages of 256 values of k (codes by TMA with the 128-byte swizzle, scales by plain bulk copies: they lie in memory
+// as the tensor cores take them), warp 1 copies a stage's scales to tensor memory and issues its MMAs, warps 2 to 9 read
+// the accumulator back.  A stage has its own columns of tensor memory for its scales, so nothing overwrites scales that
+// an MMA may still read.
+//
+// Every wait on an mbarrier has a time limit, as in gemm_tc.cu; when it runs out, the error word says which.
 #include "kernels.h"
 #include "mx4.cuh"
+#include "tc_common.cuh"
 
 namespace jb {
 
-// twice the numbers of the low halves of four bytes, as four signed bytes
-__device__ __forceinline__ int mx4_twice(uint32_t nibbles)
+constexpr int MX_TILE_M = 128;
+constexpr int MX_W_BYTES = MX_TILE_M * (MX4_CHUNK / 2);
+constexpr int MX_THREADS = 320;
+
+__device__ int g_gemm_mx4_error;    // 0, or the code of the first wait that ran out
+
+template <int BN> struct MxCfg {
+    static constexpr int A_BYTES = BN * (MX4_CHUNK / 2);
+    static constexpr int STAGE_BYTES = MX_W_BYTES + A_BYTES + 2 * MX4_TILE;
+    static constexpr int STAGES = 110 * 1024 / STAGE_BYTES > 6 ? 6 : 110 * 1024 / STAGE_BYTES;   // two CTAs fit an SM
+    static constexpr int SCALE_COL = BN < 32 ? 32 : BN;
+    static constexpr int COLS = SCALE_COL + 16 * STAGES;
+    static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */;
+};
+
+// kind::mxf4 instruction descriptor: 4-bit A and B (bits 7-9 and 10-12 = 1), both K-major, N / 8 at bit 17, scales that
+// are powers of two (bit 23), M / 16 at bit 24; which two of a column's four scales: bits 4-5 (B) and 29-30 (A).
+__host__ __device__ constexpr uint32_t mx_instr_desc(int n, int which)
 {
-    const uint32_t m = nibbles & 0x07070707u, s = (nibbles >> 3) & 0x01010101u;
-    const uint32_t sel = (m & 7) | (m >> 4 & 0x70) | (m >> 8 & 0x700) | (m >> 12 & 0x7000);
-    const uint32_t v = __byte_perm(0x03020100u, 0x0c080604u, sel);
-    const uint32_t neg = s * 255u;
-    return (int)__vsub4(v ^ neg, neg);
+    return ((uint32_t)which << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+           ((uint32_t)(MX_TILE_M >> 4) << 24) | ((uint32_t)which << 29);
+}
+
+// The descriptor of 32 rows of 16 bytes without a swizzle, 128 bytes from one group of eight rows to the next.
+__device__ __forceinline__ uint64_t mx_scale_desc(uint32_t addr)
+{
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// A stage's MMAs, by a whole warp whose lanes agree on the arguments: its scales (1,024 bytes of each operand) to tensor
+// memory, eight columns each, then four MMAs of 64 values of k.
+template <int BN>
+__device__ __forceinline__ void mx_stage(uint32_t d, uint64_t a, uint64_t b, uint32_t sa, uint32_t sb, uint64_t sa_mem,
+                                         uint64_t sb_mem, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        ".reg .b64 a1, a2, a3, b1, b2, b3, ma, mb;\n\t"
+        ".reg .b32 ta, tb;\n\t"
+        "setp.ne.b32 p, %7, 0;\n\t"
+        "add.u64 a1, %1, 2;\n\t"
+        "add.u64 a2, %1, 4;\n\t"
+        "add.u64 a3, %1, 6;\n\t"
+        "add.u64 b1, %2, 2;\n\t"
+        "add.u64 b2, %2, 4;\n\t"
+        "add.u64 b3, %2, 6;\n\t"
+        "add.u64 ma, %5, 32;\n\t"
+        "add.u64 mb, %6, 32;\n\t"
+        "add.u32 ta, %3, 4;\n\t"
+        "add.u32 tb, %4, 4;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%3], %5;\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [ta], ma;\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%4], %6;\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [tb], mb;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %8, [%3], [%4], p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %9, [%3], [%4], 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %8, [ta], [tb], 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %9, [ta], [tb], 1;\n\t"
+        "}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(sa), "r"(sb), "l"(sa_mem), "l"(sb_mem), "r"(accumulate),
+        "r"(mx_instr_desc(BN, 0)), "r"(mx_instr_desc(BN, 2))
+        : "memory");
+}
+
+__device__ __forceinline__ float4 cluster_read4(uint32_t mine, uint32_t rank)
+{
+    uint32_t ra;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(mine), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ra) : "memory");
+    return v;
+}
+
+// w_early: the weights were written before the kernel ahead of this one was launched, and may be read at once
+template <int BN, typename TO>
+__global__ void __launch_bounds__(MX_THREADS)
+gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                const uint8_t *w_scales, const uint8_t *a_scales, TO *__restrict__ out, int n, int m, int chunks, int parts,
+                int w_early)
+{
+    using Cfg = MxCfg<BN>;
+    constexpr int STAGES = Cfg::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = (uint64_t *)(smem + STAGES * Cfg::STAGE_BYTES);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 1);
+    volatile int *abort = (volatile int *)(tmem_slot + 1);
+
+    const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % parts, tile = blockIdx.x / parts;
+    const int m0 = tile * MX_TILE_M, n0 = blockIdx.y * BN;
+    const int c0 = (int)((long long)chunks * rank / parts), nc = (int)((long long)chunks * (rank + 1) / parts) - c0;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES);
+    if (threadIdx.x == 0) {
+        prefetch_tensor_map(&map_w);
+        prefetch_tensor_map(&map_a);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(accum, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = warp_uniform(*tmem_slot);
+    pdl_trigger();
+
+    const int q = warp & 3, hgrp = (warp - 2) >> 2;
+    const int rows = min(n - n0, BN);
+    bool ok = true;
+    if (warp == 0 && lane == 0) {
+        // ---------------------------------------------------------- loads
+        const uint8_t *ws = w_scales + ((size_t)tile * chunks + c0) * MX4_TILE;
+        const uint8_t *as = a_scales + ((size_t)(n0 >> 7) * chunks + c0) * MX4_TILE;
+        uint32_t armed = 0, last_parity = 0;
+        auto load_w = [&](int i, uint32_t dst, uint32_t bar) {
+            tma_load_2d(dst, &map_w, bar, (c0 + i) * (MX4_CHUNK / 2), m0);
+            bulk_load(dst + MX_W_BYTES + Cfg::A_BYTES, ws + (size_t)i * MX4_TILE, MX4_TILE, bar);
+        };
+        auto load_a = [&](int i, uint32_t dst, uint32_t bar) {
+            tma_load_2d(dst + MX_W_BYTES, &map_a, bar, (c0 + i) * (MX4_CHUNK / 2), n0);
+            bulk_load(dst + MX_W_BYTES + Cfg::A_BYTES + MX4_TILE, as + (size_t)i * MX4_TILE, MX4_TILE, bar);
+        };
+        const int pre = min(nc, STAGES);
+        if (!w_early)
+            pdl_wait();
+        for (int i = 0; i < pre; i++) {
+            mbar_expect_tx(full0 + 8 * i, Cfg::STAGE_BYTES);
+            load_w(i, smem_u32(smem + i * Cfg::STAGE_BYTES), full0 + 8 * i);
+            armed |= 1u << i;
+        }
+        if (w_early)
+            pdl_wait();
+        for (int i = 0; i < pre; i++)
+            load_a(i, smem_u32(smem + i * Cfg::STAGE_BYTES), full0 + 8 * i);
+        for (int i = pre; i < nc; i++) {
+            const int s = i % STAGES;
+            const uint32_t ph = (i / STAGES) & 1;
+            if (!mbar_wait(empty0 + 8 * s, ph ^ 1, abort, &g_gemm_mx4_error, 1))
+                break;
+            const uint32_t dst = smem_u32(smem + s * Cfg::STAGE_BYTES), bar = full0 + 8 * s;
+            mbar_expect_tx(bar, Cfg::STAGE_BYTES);
+            load_w(i, dst, bar);
+            load_a(i, dst, bar);
+            last_parity = (last_parity & ~(1u << s)) | (ph << s);
+        }
+        if (*abort) {
+            // the loads in flight: wait for each stage armed last, once, with the limit
+            volatile int never = 0;
+            for (int s = 0; s < STAGES; s++)
+                if (armed & (1u << s))
+                    mbar_wait(full0 + 8 * s, (last_parity >> s) & 1, &never, &g_gemm_mx4_error, 4);
+        }
+    } else if (warp == 1) {
+        // --------------------------------------------------------------- MMAs
+        int s = 0;
+        uint32_t ph = 0;
+        for (int i = 0; i < nc; i++) {
+            if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, ph, abort, &g_gemm_mx4_error, 2)))
+                break;
+            const uint32_t base = smem_u32(smem) + s * Cfg::STAGE_BYTES, scales = base + MX_W_BYTES + Cfg::A_BYTES;
+            const uint32_t col = tmem + Cfg::SCALE_COL + 16 * s;
+            tc_fence_after();
+            mx_stage<BN>(tmem, smem_desc_sw128(base, 16, 1024), smem_desc_sw128(base + MX_W_BYTES, 16, 1024), col, col + 8,
+                         mx_scale_desc(scales), mx_scale_desc(scales + MX4_TILE), i != 0);
+            tc_commit_warp(empty0 + 8 * s);
+            if (++s == STAGES) {
+                s = 0;
+                ph ^= 1;
+            }
+        }
+        tc_commit_warp(accum);
+    } else if (warp >= 2) {
+        // ------------------------------------------------------------ the accumulator
+        pdl_wait();
+        ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, abort, &g_gemm_mx4_error, 3));
+        tc_fence_after();
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+        const int fl = q * 32 + lane, f = m0 + fl;
+        for (int c = 8 * hgrp; c < rows && ok; c += 16) {
+            uint32_t v[8];
+            tc_ld8_nowait(taddr + c, v);
+            tc_ld_wait();
+            if (parts > 1) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (c + j < rows)
+                        ((float *)smem)[(c + j) * MX_TILE_M + fl] = __uint_as_float(v[j]);
+            } else if (f < m) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (c + j < rows)
+                        out[(size_t)(n0 + c + j) * m + f] = from_f<TO>(__uint_as_float(v[j]));
+            }
+        }
+    }
+    if (parts > 1) {
+        // ---------------------------------------------------------- the parts' sums, in the order of k
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (warp >= 2) {
+            const bool vec = m % 4 == 0;
+            for (int g = rank * (MX_THREADS - 64) + (int)threadIdx.x - 64; g < rows * (MX_TILE_M / 4); g += parts * (MX_THREADS - 64)) {
+                const uint32_t at = smem_u32(smem) + g * 16;
+                float4 t = cluster_read4(at, 0);
+                for (int p = 1; p < parts; p++) {
+                    const float4 u = cluster_read4(at, p);
+                    t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+                }
+                const int f = m0 + (g % (MX_TILE_M / 4)) * 4;
+                TO *o = out + (size_t)(n0 + g / (MX_TILE_M / 4)) * m + f;
+                if (vec) {
+                    if (f < m)
+                        store4(o, t);
+                } else {
+                    if (f < m)
+                        o[0] = from_f<TO>(t.x);
+                    if (f + 1 < m)
+                        o[1] = from_f<TO>(t.y);
+                    if (f + 2 < m)
+                        o[2] = from_f<TO>(t.z);
+                    if (f + 3 < m)
+                        o[3] = from_f<TO>(t.w);
+                }
+            }
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();             // no CTA ends while another reads its sums
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                     ::"r"(tmem), "r"((uint32_t)Cfg::TMEM_COLS) : "memory");
+}
+
+// A matrix of codes in boxes of box_rows x 128 bytes with the 128-byte swizzle; what lies outside reads as zero.
+static bool mx_tensor_map(const void *codes, int rows, int k, int box_rows, CUtensorMap *out)
+{
+    EncodeTiled enc = tensor_map_encoder();
+    if (!enc)
+        return false;
+    cuuint64_t dims[2] = {(cuuint64_t)mx4_row_bytes(k), (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)mx4_row_bytes(k)};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Parts of k (1, 2, 4 or 8) that a product's tiles are shared out in.
+static int mx_parts(int tiles, int chunks)
+{
+    int p = 1;
+    while (p < 8 && tiles * p * 2 <= 2 * sm_count() && p * 2 <= chunks)
+        p *= 2;
+    return p;
+}
+
+template <int BN, typename TO>
+static int launch_mx(const void *ac, const void *as, const void *wc, const void *ws, TO *out, int n, int m, int k, int w_early,
+                     cudaStream_t st)
+{
+    using Cfg = MxCfg<BN>;
+    CUtensorMap map_w, map_a;
+    if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || !mx_tensor_map(ac, n, k, BN, &map_a))
+        return JB_EINVAL;
+    auto kern = gemm_mx4_kernel<BN, TO>;
+    static unsigned long long allowed = 0;
+    if (!allow_dynamic_smem(kern, Cfg::SMEM_BYTES, allowed))
+        return JB_ELAUNCH;
+    const int tiles_m = (m + MX_TILE_M - 1) / MX_TILE_M, tiles_n = (n + BN - 1) / BN, chunks = mx4_chunks(k);
+    if (tiles_n > 65535)
+        return JB_EINVAL;
+    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks);
+    launch_cluster(kern, dim3((unsigned)tiles_m * parts, tiles_n), MX_THREADS, Cfg::SMEM_BYTES, st, (unsigned)parts, map_w,
+                   map_a, (const uint8_t *)ws, (const uint8_t *)as, out, n, m, chunks, parts, w_early);
+    return launch_status();
 }
 
 template <typename TO>
-__global__ void __launch_bounds__(256)
-mx4_product_kernel(const uint8_t *ac, const uint8_t *as, const uint8_t *wc, const uint8_t *ws, TO *__restrict__ out, int n,
-                   int m, int k)
+static int any_mx(const void *ac, const void *as, const void *wc, const void *ws, TO *out, int n, int m, int k, int w_early,
+                  cudaStream_t st)
 {
-    pdl_trigger();
-    pdl_wait();
-    const int f = blockIdx.y * 32 + (threadIdx.x & 31);
-    const size_t r = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (f >= m || r >= (size_t)n)
-        return;
-    const size_t row_bytes = mx4_row_bytes(k);
-    const int chunks = mx4_chunks(k), blocks = (k + 31) / 32;
-    float sum = 0.0f;
-    for (int b = 0; b < blocks; b++) {
-        const uint4 a = *reinterpret_cast<const uint4 *>(ac + r * row_bytes + (size_t)b * 16);
-        const uint4 w = *reinterpret_cast<const uint4 *>(wc + (size_t)f * row_bytes + (size_t)b * 16);
-        const uint32_t av[4] = {a.x, a.y, a.z, a.w}, wv[4] = {w.x, w.y, w.z, w.w};
-        int dot = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            dot = __dp4a(mx4_twice(av[i]), mx4_twice(wv[i]), dot);
-            dot = __dp4a(mx4_twice(av[i] >> 4), mx4_twice(wv[i] >> 4), dot);
-        }
-        const int half = (b >> 2) & 1, q = b & 3;
-        const float sa = mx4_scale(as[mx4_scale_at(r, b >> 3, chunks, half) + q]);
-        const float sw = mx4_scale(ws[mx4_scale_at(f, b >> 3, chunks, half) + q]);
-        sum += 0.25f * (float)dot * sa * sw;
-    }
-    out[r * m + f] = from_f<TO>(sum);
+    if (n <= 16)
+        return launch_mx<16, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 32)
+        return launch_mx<32, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 64)
+        return launch_mx<64, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+    return launch_mx<128, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
 }
 
 }  // namespace jb
 
 using namespace jb;
 
-// out [n, m] (out_dt 0 float32, 1 bfloat16) = a [n, k] . w [m, k]^T, both as codes and scales.
+// out [n, m] (out_dt 0 float32, 1 bfloat16) = a [n, k] . w [m, k]^T, both as codes and scales.  w_early: no kernel that
+// may still be running when this one starts writes the weights.
 extern "C" int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales, void *out,
-                             int out_dt, int n, int m, int k, cudaStream_t st)
+                             int out_dt, int n, int m, int k, int w_early, cudaStream_t st)
 {
     if (n < 0 || m < 0 || k < 1 || (out_dt != 0 && out_dt != 1) || (uintptr_t)a_codes % 16 || (uintptr_t)w_codes % 16 ||
-        (uintptr_t)a_scales % 16 || (uintptr_t)w_scales % 16 || (m + 31) / 32 > 65535)
+        (uintptr_t)a_scales % 16 || (uintptr_t)w_scales % 16)
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;
-    const dim3 grid((unsigned)((n + 7) / 8), (unsigned)((m + 31) / 32));
-    if (out_dt == 1)
-        launch(mx4_product_kernel<bf16>, grid, 256, 0, st, (const uint8_t *)a_codes, (const uint8_t *)a_scales,
-               (const uint8_t *)w_codes, (const uint8_t *)w_scales, (bf16 *)out, n, m, k);
-    else
-        launch(mx4_product_kernel<float>, grid, 256, 0, st, (const uint8_t *)a_codes, (const uint8_t *)a_scales,
-               (const uint8_t *)w_codes, (const uint8_t *)w_scales, (float *)out, n, m, k);
-    return launch_status();
+    return out_dt == 1 ? any_mx(a_codes, a_scales, w_codes, w_scales, (bf16 *)out, n, m, k, w_early, st)
+                       : any_mx(a_codes, a_scales, w_codes, w_scales, (float *)out, n, m, k, w_early, st);
+}
+
+// Reads and clears the error word: 0, or which wait ran out first (as jb_gemm_tc_error).
+extern "C" int jb_gemm_mx4_error(void)
+{
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_gemm_mx4_error, sizeof v) != cudaSuccess)
+        return JB_ELAUNCH;
+    if (v != 0)
+        cudaMemcpyToSymbol(g_gemm_mx4_error, &zero, sizeof zero);
+    return v;
 }

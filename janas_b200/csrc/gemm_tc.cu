@@ -712,7 +712,7 @@ extern "C" int jb_gemm_tc_gated(const void *A, const void *W, void *out_act, int
 
 // Reads and clears the error words of the products: 0, or which wait ran out first (1: a free
 // stage, 2: a loaded stage, 3: the accumulator, 4: a load in flight; from 20 on: in the product of
-// floats, gemm_f32_tc.cu).
+// floats, gemm_f32_tc.cu; from 40 on: in the product of 4-bit floats, gemm_mx4.cu).
 // Synchronizes the device.
 // A wait that nothing ends, to show that a bounded wait runs out as it should: one
 // warp, one mbarrier that no thread and no copy ever arrives at, the products' own
@@ -754,6 +754,6 @@ extern "C" int jb_gemm_tc_error(void)
         return JB_ELAUNCH;
     if (v != 0)
         cudaMemcpyToSymbol(g_gemm_tc_error, &zero, sizeof zero);
-    int f = jb_gemm_f32_tc_error();
-    return v != 0 ? v : f > 0 ? f + 20 : f;
+    int f = jb_gemm_f32_tc_error(), x = jb_gemm_mx4_error();
+    return v != 0 ? v : f > 0 ? f + 20 : f != 0 ? f : x > 0 ? x + 40 : x;
 }

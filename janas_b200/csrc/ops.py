@@ -1428,7 +1428,7 @@ def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tenso
     n, m = a.rows, w.rows
     out = torch.empty((n, m), dtype=out_dtype, device=w.codes.device)
     _check(lib().jb_linear_mx4(_p(a.codes), _p(a.scales), _p(w.codes), _p(w.scales), _p(out), _DT[out_dtype], n, m, w.k,
-                               _stream()), "linear_mx4", 1 if n and m else 0)
+                               1 if w.settled else 0, _stream()), "linear_mx4", 1 if n and m else 0)
     return out
 
 
