@@ -12,6 +12,9 @@
 // the accumulator back.  A stage has its own columns of tensor memory for its scales, so nothing overwrites scales that
 // an MMA may still read.
 //
+// Up to 32 rows may come as floats: every CTA then brings its part of them to 4 bits itself (warps 2 to 9, a warp a row's
+// chunk, the next four chunks' loads in flight), which costs less than the launch of a kernel that does it once.
+//
 // Every wait on an mbarrier has a time limit, as in gemm_tc.cu; when it runs out, the error word says which.
 #include "kernels.h"
 #include "mx4.cuh"
@@ -101,12 +104,31 @@ __device__ __forceinline__ float4 cluster_read4(uint32_t mine, uint32_t rank)
     return v;
 }
 
+// Rows as floats in memory: [n, k] of bfloat16 or float, vec: whole 16-byte loads.
+struct MxRows {
+    const void *x;
+    int k, is_bf16, vec;
+};
+
+// Eight values of row r from column col on, zeros past the row's end.
+__device__ __forceinline__ void mx_fetch(const MxRows &a, size_t r, int col, float *v)
+{
+    const size_t at = r * (size_t)a.k + col;
+    if (a.is_bf16) {
+        const bf16 *p = (const bf16 *)a.x + at;
+        a.vec ? load8<bf16, true>(p, a.k - col, v) : load8<bf16, false>(p, a.k - col, v);
+    } else {
+        const float *p = (const float *)a.x + at;
+        a.vec ? load8<float, true>(p, a.k - col, v) : load8<float, false>(p, a.k - col, v);
+    }
+}
+
 // w_early: the weights were written before the kernel ahead of this one was launched, and may be read at once
-template <int BN, typename TO>
+template <int BN, typename TO, bool ROWS>
 __global__ void __launch_bounds__(MX_THREADS)
 gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
-                const uint8_t *w_scales, const uint8_t *a_scales, TO *__restrict__ out, int n, int m, int chunks, int parts,
-                int w_early)
+                const uint8_t *w_scales, const uint8_t *a_scales, const MxRows a_rows, TO *__restrict__ out, int n, int m,
+                int chunks, int parts, int w_early)
 {
     using Cfg = MxCfg<BN>;
     constexpr int STAGES = Cfg::STAGES;
@@ -123,9 +145,10 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES);
     if (threadIdx.x == 0) {
         prefetch_tensor_map(&map_w);
-        prefetch_tensor_map(&map_a);
+        if (!ROWS)
+            prefetch_tensor_map(&map_a);
         for (int s = 0; s < STAGES; s++) {
-            mbar_init(full0 + 8 * s, 1);
+            mbar_init(full0 + 8 * s, ROWS ? 9 : 1);        // the loads, and the warps that pack the rows
             mbar_init(empty0 + 8 * s, 1);
         }
         mbar_init(accum, 1);
@@ -145,6 +168,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
     const int q = warp & 3, hgrp = (warp - 2) >> 2;
     const int rows = min(n - n0, BN);
+    constexpr uint32_t LOADED = ROWS ? MX_W_BYTES + MX4_TILE : Cfg::STAGE_BYTES;
     bool ok = true;
     if (warp == 0 && lane == 0) {
         // ---------------------------------------------------------- loads
@@ -163,13 +187,13 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (!w_early)
             pdl_wait();
         for (int i = 0; i < pre; i++) {
-            mbar_expect_tx(full0 + 8 * i, Cfg::STAGE_BYTES);
+            mbar_expect_tx(full0 + 8 * i, LOADED);
             load_w(i, smem_u32(smem + i * Cfg::STAGE_BYTES), full0 + 8 * i);
             armed |= 1u << i;
         }
-        if (w_early)
+        if (w_early && !ROWS)
             pdl_wait();
-        for (int i = 0; i < pre; i++)
+        for (int i = 0; i < pre && !ROWS; i++)
             load_a(i, smem_u32(smem + i * Cfg::STAGE_BYTES), full0 + 8 * i);
         for (int i = pre; i < nc; i++) {
             const int s = i % STAGES;
@@ -177,9 +201,10 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             if (!mbar_wait(empty0 + 8 * s, ph ^ 1, abort, &g_gemm_mx4_error, 1))
                 break;
             const uint32_t dst = smem_u32(smem + s * Cfg::STAGE_BYTES), bar = full0 + 8 * s;
-            mbar_expect_tx(bar, Cfg::STAGE_BYTES);
+            mbar_expect_tx(bar, LOADED);
             load_w(i, dst, bar);
-            load_a(i, dst, bar);
+            if (!ROWS)
+                load_a(i, dst, bar);
             last_parity = (last_parity & ~(1u << s)) | (ph << s);
         }
         if (*abort) {
@@ -211,6 +236,45 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     } else if (warp >= 2) {
         // ------------------------------------------------------------ the accumulator
         pdl_wait();
+        if constexpr (ROWS) {
+            // item t: chunk t / groups of row (warp - 2) + 8 (t % groups)
+            constexpr int AHEAD = 4;
+            const int groups = (rows + 7) / 8, items = nc * groups;
+            float v[AHEAD][8];
+            auto fetch = [&](int t, float *to) {
+                const int i = t / groups, r = warp - 2 + 8 * (t - i * groups);
+                if (t < items && r < rows)
+                    mx_fetch(a_rows, r, (c0 + i) * MX4_CHUNK + 8 * lane, to);
+            };
+#pragma unroll
+            for (int d = 0; d < AHEAD; d++)
+                fetch(d, v[d]);
+            for (int t0 = 0; t0 < items && ok; t0 += AHEAD) {
+#pragma unroll
+                for (int d = 0; d < AHEAD; d++) {
+                    const int t = t0 + d, i = t / groups, g = t - i * groups, s = i % STAGES, r = warp - 2 + 8 * g;
+                    if (t >= items || !ok)
+                        continue;
+                    if (g == 0 && i >= STAGES)
+                        ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / STAGES) & 1) ^ 1, abort, &g_gemm_mx4_error, 5));
+                    uint8_t *stage = smem + s * Cfg::STAGE_BYTES + MX_W_BYTES;
+                    if (ok && r < rows) {
+                        uint32_t word;
+                        const uint32_t packed = mx4_pack_chunk(v[d], word);
+                        *reinterpret_cast<uint32_t *>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = packed;
+                        if ((lane & 15) == 0)
+                            *reinterpret_cast<uint32_t *>(stage + Cfg::A_BYTES + MX4_TILE + (lane >> 4) * 512 + r * 16) = word;
+                    }
+                    fetch(t + AHEAD, v[d]);
+                    if (ok && g == groups - 1) {
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0)
+                            mbar_arrive(full0 + 8 * s);
+                    }
+                }
+            }
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, abort, &g_gemm_mx4_error, 3));
         tc_fence_after();
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
@@ -297,15 +361,17 @@ static int mx_parts(int tiles, int chunks)
     return p;
 }
 
-template <int BN, typename TO>
-static int launch_mx(const void *ac, const void *as, const void *wc, const void *ws, TO *out, int n, int m, int k, int w_early,
-                     cudaStream_t st)
+template <int BN, typename TO, bool ROWS>
+static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, int n, int m, int k,
+                     int w_early, cudaStream_t st)
 {
     using Cfg = MxCfg<BN>;
     CUtensorMap map_w, map_a;
-    if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || !mx_tensor_map(ac, n, k, BN, &map_a))
+    if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || (!ROWS && !mx_tensor_map(ac, n, k, BN, &map_a)))
         return JB_EINVAL;
-    auto kern = gemm_mx4_kernel<BN, TO>;
+    if (ROWS)
+        map_a = map_w;              // not used
+    auto kern = gemm_mx4_kernel<BN, TO, ROWS>;
     static unsigned long long allowed = 0;
     if (!allow_dynamic_smem(kern, Cfg::SMEM_BYTES, allowed))
         return JB_ELAUNCH;
@@ -314,21 +380,32 @@ static int launch_mx(const void *ac, const void *as, const void *wc, const void 
         return JB_EINVAL;
     const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks);
     launch_cluster(kern, dim3((unsigned)tiles_m * parts, tiles_n), MX_THREADS, Cfg::SMEM_BYTES, st, (unsigned)parts, map_w,
-                   map_a, (const uint8_t *)ws, (const uint8_t *)as, out, n, m, chunks, parts, w_early);
+                   map_a, (const uint8_t *)ws, (const uint8_t *)as, rows, out, n, m, chunks, parts, w_early);
     return launch_status();
 }
 
+constexpr int MX_ROWS_MOST = 32;    // rows that the product takes as floats
+
 template <typename TO>
-static int any_mx(const void *ac, const void *as, const void *wc, const void *ws, TO *out, int n, int m, int k, int w_early,
-                  cudaStream_t st)
+static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, int n, int m, int k,
+                  int w_early, cudaStream_t st)
 {
+    if (rows.x)
+        return n <= 16 ? launch_mx<16, TO, true>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
+                       : launch_mx<32, TO, true>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 16)
-        return launch_mx<16, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+        return launch_mx<16, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 32)
-        return launch_mx<32, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+        return launch_mx<32, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 64)
-        return launch_mx<64, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
-    return launch_mx<128, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+        return launch_mx<64, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    return launch_mx<128, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+}
+
+static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, int out_dt, int n, int m, int k)
+{
+    return n < 0 || m < 0 || k < 1 || (out_dt != 0 && out_dt != 1) || (uintptr_t)ac % 16 || (uintptr_t)as % 16 ||
+           (uintptr_t)wc % 16 || (uintptr_t)ws % 16;
 }
 
 }  // namespace jb
@@ -340,13 +417,38 @@ using namespace jb;
 extern "C" int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales, void *out,
                              int out_dt, int n, int m, int k, int w_early, cudaStream_t st)
 {
-    if (n < 0 || m < 0 || k < 1 || (out_dt != 0 && out_dt != 1) || (uintptr_t)a_codes % 16 || (uintptr_t)w_codes % 16 ||
-        (uintptr_t)a_scales % 16 || (uintptr_t)w_scales % 16)
+    if (bad_product(a_codes, a_scales, w_codes, w_scales, out_dt, n, m, k))
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;
-    return out_dt == 1 ? any_mx(a_codes, a_scales, w_codes, w_scales, (bf16 *)out, n, m, k, w_early, st)
-                       : any_mx(a_codes, a_scales, w_codes, w_scales, (float *)out, n, m, k, w_early, st);
+    const MxRows none{nullptr, k, 0, 0};
+    return out_dt == 1 ? any_mx(a_codes, a_scales, none, w_codes, w_scales, (bf16 *)out, n, m, k, w_early, st)
+                       : any_mx(a_codes, a_scales, none, w_codes, w_scales, (float *)out, n, m, k, w_early, st);
+}
+
+// The most rows that jb_linear_mx4_rows needs no scratch for.
+extern "C" int jb_linear_mx4_rows_most(void) { return MX_ROWS_MOST; }
+
+// The same with a as floats (dt 0 float32, 1 bfloat16), which are brought to 4 bits on the way: in the product's own
+// kernel for up to jb_linear_mx4_rows_most() rows, else by a kernel ahead of it, in scratch (jb_mx4_code_bytes and
+// jb_mx4_scale_bytes of [n, k], one behind the other).
+extern "C" int jb_linear_mx4_rows(const void *x, int dt, void *scratch, const void *w_codes, const void *w_scales, void *out,
+                                  int out_dt, int n, int m, int k, int w_early, cudaStream_t st)
+{
+    if (bad_product(scratch, nullptr, w_codes, w_scales, out_dt, n, m, k) || (dt != 0 && dt != 1))
+        return JB_EINVAL;
+    if (n == 0 || m == 0)
+        return JB_OK;
+    if (n > MX_ROWS_MOST) {
+        if (!scratch)
+            return JB_EINVAL;
+        void *scales = (uint8_t *)scratch + jb_mx4_code_bytes(n, k);
+        const int e = jb_mx4_quantize(x, dt, scratch, scales, n, k, 1, st);
+        return e != JB_OK ? e : jb_linear_mx4(scratch, scales, w_codes, w_scales, out, out_dt, n, m, k, w_early, st);
+    }
+    const MxRows rows{x, k, dt, k % 8 == 0 && (uintptr_t)x % 16 == 0};
+    return out_dt == 1 ? any_mx(nullptr, nullptr, rows, w_codes, w_scales, (bf16 *)out, n, m, k, w_early, st)
+                       : any_mx(nullptr, nullptr, rows, w_codes, w_scales, (float *)out, n, m, k, w_early, st);
 }
 
 // Reads and clears the error word: 0, or which wait ran out first (as jb_gemm_tc_error).

@@ -11,31 +11,18 @@
 
 namespace jb {
 
-// Eight consecutive values of a row from column col0 on; zeros past the row's end.
 template <typename T, bool VEC> struct RowSource {
     const T *x;
     int k;
     __device__ __forceinline__ void load(size_t r, int col0, float *v) const
     {
-        const T *p = x + r * (size_t)k + col0;
-        if (VEC) {
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-            if (col0 < k) {
-                a = load4(p);
-                b = load4(p + 4);
-            }
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                v[i] = col0 + i < k ? to_f(p[i]) : 0.0f;
-        }
+        load8<T, VEC>(x + r * (size_t)k + col0, k - col0, v);
     }
+    __device__ __forceinline__ void finish(float *) const {}
 };
 
 // The gated unit of the sums [S, n, 2 k]: columns [0, k) the gate, [k, 2 k) the up side.
-struct UnitSource {
+template <bool VEC> struct UnitSource {
     const float *z;
     int S;
     size_t stride;
@@ -44,61 +31,121 @@ struct UnitSource {
     __device__ __forceinline__ void load(size_t r, int col0, float *v) const
     {
         const float *g = z + r * 2 * (size_t)k + col0, *u = g + k;
+        load8<float, VEC>(g, k - col0, v);
+        load8<float, VEC>(u, k - col0, v + 8);
+        for (int s = 1; s < S; s++) {
+            float t[16];
+            load8<float, VEC>(g + s * stride, k - col0, t);
+            load8<float, VEC>(u + s * stride, k - col0, t + 8);
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                v[i] += t[i];
+        }
+    }
+    __device__ __forceinline__ void finish(float *v) const
+    {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            v[i] = col0 + i < k ? gated_unit(add_partials(0.0f, g + i, S, stride), add_partials(0.0f, u + i, S, stride), unit)
-                                : 0.0f;
+            v[i] = gated_unit(v[i], v[8 + i], unit);
     }
 };
 
-template <typename Source>
+// Every warp takes U chunks that follow one another, all read before the first is packed: what is in flight decides the
+// bandwidth, and few rows are better spread over many warps (U = 1).  `total`: n times the chunks of a row.
+template <typename Source, int U, int VALUES>
 __global__ void __launch_bounds__(256)
-mx4_quantize_kernel(const Source src, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, int n, int k, int early)
+mx4_quantize_kernel(const Source src, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, unsigned total, int k, int early)
 {
     if (early)
         pdl_trigger();
     pdl_wait();
-    const int chunks = mx4_chunks(k);
-    const size_t total = (size_t)n * chunks, step = (size_t)gridDim.x * (blockDim.x >> 5);
-    for (size_t i = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += step) {
-        const size_t r = i / chunks;
-        const int c = (int)(i - r * chunks);
-        float v[8];
-        src.load(r, c * MX4_CHUNK + 8 * (threadIdx.x & 31), v);
-        mx4_store_chunk(v, r, c, k, codes, scales);
+    const unsigned chunks = mx4_chunks(k), first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * U;
+    float v[U][VALUES];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const unsigned i = first + u, r = i / chunks;
+        if (i < total)
+            src.load(r, (i - r * chunks) * MX4_CHUNK + 8 * (threadIdx.x & 31), v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const unsigned i = first + u, r = i / chunks;
+        if (i < total) {
+            src.finish(v[u]);
+            mx4_store_chunk(v[u], r, i - r * chunks, k, codes, scales);
+        }
     }
     if (!early)
         __threadfence();
 }
 
-template <typename T>
+template <typename T, int U, bool VEC>
 __global__ void __launch_bounds__(256)
-mx4_values_kernel(const uint8_t *codes, const uint8_t *scales, T *__restrict__ out, int n, int k)
+mx4_values_kernel(const uint8_t *codes, const uint8_t *scales, T *__restrict__ out, unsigned total, int k)
 {
     pdl_trigger();
     pdl_wait();
-    const int chunks = mx4_chunks(k), lane = threadIdx.x & 31;
-    const size_t total = (size_t)n * chunks, step = (size_t)gridDim.x * (blockDim.x >> 5), row_bytes = mx4_row_bytes(k);
-    for (size_t i = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += step) {
-        const size_t r = i / chunks;
-        const int c = (int)(i - r * chunks), col0 = c * MX4_CHUNK + 8 * lane;
-        if (col0 >= k)
+    const unsigned chunks = mx4_chunks(k), first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * U;
+    const int lane = threadIdx.x & 31;
+    const size_t row_bytes = mx4_row_bytes(k);
+    uint32_t word[U], scale[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const unsigned i = first + u, r = i / chunks, c = i - r * chunks;
+        const int col0 = c * MX4_CHUNK + 8 * lane;
+        if (i < total && col0 < k) {
+            word[u] = *reinterpret_cast<const uint32_t *>(codes + r * row_bytes + col0 / 2);
+            scale[u] = scales[mx4_scale_at(r, c, chunks, lane >> 4) + ((lane >> 2) & 3)];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const unsigned i = first + u, r = i / chunks, c = i - r * chunks;
+        const int col0 = c * MX4_CHUNK + 8 * lane;
+        if (i >= total || col0 >= k)
             continue;
         float v[8];
-        mx4_unpack8(*reinterpret_cast<const uint32_t *>(codes + r * row_bytes + col0 / 2), v);
-        const float s = mx4_scale(scales[mx4_scale_at(r, c, chunks, lane >> 4) + ((lane >> 2) & 3)]);
+        mx4_unpack8(word[u], v);
+        const float s = mx4_scale(scale[u]);
         T *o = out + r * (size_t)k + col0;
+        if (VEC) {
+            store4(o, make_float4(v[0] * s, v[1] * s, v[2] * s, v[3] * s));
+            store4(o + 4, make_float4(v[4] * s, v[5] * s, v[6] * s, v[7] * s));
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (col0 + j < k)
-                o[j] = from_f<T>(v[j] * s);
+            for (int j = 0; j < 8; j++)
+                if (col0 + j < k)
+                    o[j] = from_f<T>(v[j] * s);
+        }
     }
 }
 
-static unsigned warps_grid(size_t chunks)
+// Chunks that a warp takes: four once that leaves all SMs 32 warps.
+static int mx4_unroll(size_t total) { return total >= (size_t)sm_count() * 32 * 4 ? 4 : 1; }
+static unsigned mx4_grid(size_t total, int unroll) { return (unsigned)((total + 8 * unroll - 1) / (8 * unroll)); }
+
+template <typename Source, int VALUES>
+static int quantize(const Source &src, void *codes, void *scales, int n, int k, int early, cudaStream_t st)
 {
-    const size_t blocks = (chunks + 7) / 8, most = (size_t)sm_count() * 8;
-    return (unsigned)(blocks < most ? blocks : most);
+    const size_t total = (size_t)n * mx4_chunks(k);
+    if (total > 0xffffff00u)
+        return JB_EINVAL;
+    const int u = mx4_unroll(total);
+    launch(u == 4 ? mx4_quantize_kernel<Source, 4, VALUES> : mx4_quantize_kernel<Source, 1, VALUES>, mx4_grid(total, u), 256, 0,
+           st, src, (uint8_t *)codes, (uint8_t *)scales, (unsigned)total, k, early);
+    return launch_status();
+}
+
+template <typename T, bool VEC>
+static int values(const void *codes, const void *scales, T *out, int n, int k, cudaStream_t st)
+{
+    const size_t total = (size_t)n * mx4_chunks(k);
+    if (total > 0xffffff00u)
+        return JB_EINVAL;
+    const int u = mx4_unroll(total);
+    launch(u == 4 ? mx4_values_kernel<T, 4, VEC> : mx4_values_kernel<T, 1, VEC>, mx4_grid(total, u), 256, 0, st,
+           (const uint8_t *)codes, (const uint8_t *)scales, out, (unsigned)total, k);
+    return launch_status();
 }
 
 }  // namespace jb
@@ -125,16 +172,11 @@ extern "C" int jb_mx4_quantize(const void *x, int dt, void *codes, void *scales,
     if (n == 0)
         return JB_OK;
     const bool vec = k % 8 == 0 && (uintptr_t)x % 16 == 0;
-    const unsigned grid = warps_grid((size_t)n * mx4_chunks(k));
-#define JB_Q(T, V) \
-    launch(mx4_quantize_kernel<RowSource<T, V>>, grid, 256, 0, st, RowSource<T, V>{(const T *)x, k}, (uint8_t *)codes, \
-           (uint8_t *)scales, n, k, early)
+#define JB_Q(T, V) quantize<RowSource<T, V>, 8>(RowSource<T, V>{(const T *)x, k}, codes, scales, n, k, early, st)
     if (dt == 1)
-        vec ? JB_Q(bf16, true) : JB_Q(bf16, false);
-    else
-        vec ? JB_Q(float, true) : JB_Q(float, false);
+        return vec ? JB_Q(bf16, true) : JB_Q(bf16, false);
+    return vec ? JB_Q(float, true) : JB_Q(float, false);
 #undef JB_Q
-    return launch_status();
 }
 
 // The gated unit (see jb_gated_unit) of z, a stack [S, n, 2 ff] of sums, in 4 bits.
@@ -145,9 +187,10 @@ extern "C" int jb_mx4_gated_unit(const float *z, int S, long long stride, void *
         return JB_EINVAL;
     if (n == 0)
         return JB_OK;
-    launch(mx4_quantize_kernel<UnitSource>, warps_grid((size_t)n * mx4_chunks(ff)), 256, 0, st,
-           UnitSource{z, S, (size_t)stride, ff, GatedUnit{alpha, limit, shift}}, (uint8_t *)codes, (uint8_t *)scales, n, ff, 1);
-    return launch_status();
+    const GatedUnit unit{alpha, limit, shift};
+    if (ff % 8 == 0 && (uintptr_t)z % 16 == 0 && stride % 4 == 0)
+        return quantize<UnitSource<true>, 16>(UnitSource<true>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
+    return quantize<UnitSource<false>, 16>(UnitSource<false>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
 }
 
 // What codes and scales stand for, as [n, k].
@@ -157,10 +200,10 @@ extern "C" int jb_mx4_values(const void *codes, const void *scales, void *out, i
         return JB_EINVAL;
     if (n == 0)
         return JB_OK;
-    const unsigned grid = warps_grid((size_t)n * mx4_chunks(k));
+    const bool vec = k % 8 == 0 && (uintptr_t)out % 16 == 0;
     if (out_dt == 1)
-        launch(mx4_values_kernel<bf16>, grid, 256, 0, st, (const uint8_t *)codes, (const uint8_t *)scales, (bf16 *)out, n, k);
-    else
-        launch(mx4_values_kernel<float>, grid, 256, 0, st, (const uint8_t *)codes, (const uint8_t *)scales, (float *)out, n, k);
-    return launch_status();
+        return vec ? values<bf16, true>(codes, scales, (bf16 *)out, n, k, st)
+                   : values<bf16, false>(codes, scales, (bf16 *)out, n, k, st);
+    return vec ? values<float, true>(codes, scales, (float *)out, n, k, st)
+               : values<float, false>(codes, scales, (float *)out, n, k, st);
 }

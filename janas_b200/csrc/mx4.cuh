@@ -75,24 +75,57 @@ __device__ __forceinline__ uint32_t mx4_top8(const float *v)
     return t;
 }
 
-// A warp packs a row's chunk of 256 values, eight to a lane (zeros past the row's end): codes and scales to memory.
+// Eight consecutive floats of which `left` exist; zeros for the others.  VEC: all eight or none, at a 16-byte boundary.
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *p, int left, float *v)
+{
+    if (VEC) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (left > 0) {
+            if (sizeof(T) == 2) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(p);
+                a = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                                __uint_as_float(u.y & 0xffff0000u));
+                b = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xffff0000u), __uint_as_float(u.w << 16),
+                                __uint_as_float(u.w & 0xffff0000u));
+            } else {
+                a = load4(p);
+                b = load4(p + 4);
+            }
+        }
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            v[i] = i < left ? to_f(p[i]) : 0.0f;
+    }
+}
+
+// A warp packs a chunk of 256 values, eight to a lane (zeros past the row's end): the lane's codes, and in lanes 0 and 16
+// the scales' codes of the four blocks of their half of the chunk.
+__device__ __forceinline__ uint32_t mx4_pack_chunk(const float *v, uint32_t &word)
+{
+    uint32_t top = mx4_top8(v);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t code = mx4_scale_code(top);
+    word = code;
+    word |= __shfl_down_sync(0xffffffffu, code, 4) << 8;
+    word |= __shfl_down_sync(0xffffffffu, code, 8) << 16;
+    word |= __shfl_down_sync(0xffffffffu, code, 12) << 24;
+    return mx4_pack8(v, mx4_inverse(code));
+}
+
+// The same, to memory: chunk c of row r.
 __device__ __forceinline__ void mx4_store_chunk(const float *v, size_t r, int c, int k, uint8_t *__restrict__ codes,
                                                 uint8_t *__restrict__ scales)
 {
     const int lane = threadIdx.x & 31;
-    uint32_t top = mx4_top8(v);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    uint32_t code = mx4_scale_code(top);
-    uint32_t packed = mx4_pack8(v, mx4_inverse(code));
+    uint32_t word;
+    const uint32_t packed = mx4_pack_chunk(v, word);
     const size_t row_bytes = mx4_row_bytes(k), at = (size_t)c * (MX4_CHUNK / 2) + lane * 4;
     if (at < row_bytes)
         *reinterpret_cast<uint32_t *>(codes + r * row_bytes + at) = packed;
-    // the codes of four blocks in one word: lanes 0, 4, 8, 12 of this half of the warp
-    uint32_t word = code;
-    word |= __shfl_down_sync(0xffffffffu, code, 4) << 8;
-    word |= __shfl_down_sync(0xffffffffu, code, 8) << 16;
-    word |= __shfl_down_sync(0xffffffffu, code, 12) << 24;
     if ((lane & 15) == 0)
         *reinterpret_cast<uint32_t *>(scales + mx4_scale_at(r, c, mx4_chunks(k), lane >> 4)) = word;
 }

@@ -483,33 +483,34 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
     n, dm = x.shape
     y = stack(y)
     _need(y, "y", torch.float32, (None, n, dm))
-    at = x.device
+    here = x.get_device()
+    vectors, vec = [], (dm,)
     for t, name in ((y_bias, "y_bias"), (gate_bias, "gate_bias"), (post_weight, "post_weight"), (post_bias, "post_bias"),
-                    (next_weight, "next_weight"), (next_bias, "next_bias")):
-        if t is not None:
-            _need(t, name, torch.float32, (dm,))
-            if t.device != at:
-                raise KernelError(f"{name}: on another device than x")
-    Sg, g_ld = 0, 0
+                    (next_weight, "next_weight"), (next_bias, "next_bias"),
+                    (scale if scale.__class__ is not float else None, "scale")):
+        if t is None or t.__class__ is int:
+            vectors.append(None)
+            continue
+        _need(t, name, torch.float32, vec)
+        if t.get_device() != here:
+            raise KernelError(f"{name}: on another device than x")
+        vectors.append(t.data_ptr())
+    Sg, g_ld, gate = 0, 0, None
     if y_gate is not None:
         y_gate = stack(y_gate)
         _need(y_gate, "y_gate", torch.float32, (None, n, None))
         Sg, _, g_ld = y_gate.shape
-        if Sg < 1 or gate_col0 < 0 or g_ld - gate_col0 < dm or y_gate.device != at:
+        if Sg < 1 or gate_col0 < 0 or g_ld - gate_col0 < dm or y_gate.get_device() != here:
             raise KernelError("norm_residual_norm: the gate's columns lie outside y_gate, or it is on another device")
+        gate = y_gate.data_ptr()
     elif gate_bias is not None:
         raise KernelError("norm_residual_norm: a gate_bias without a gate")
     if (post_bias is not None and post_weight is None) or (next_bias is not None and next_weight is None):
         raise KernelError("norm_residual_norm: a norm's bias without its weight")
-    if not y.shape[0] or y.device != at:
+    S = y.shape[0]
+    if not S or y.get_device() != here:
         raise KernelError("norm_residual_norm: y needs at least one sum, on x's device")
-    mult = 1.0
-    if isinstance(scale, torch.Tensor):
-        _need(scale, "scale", torch.float32, (dm,))
-        if scale.device != at:
-            raise KernelError("scale: on another device than x")
-    elif scale is not None:
-        mult, scale = float(scale), None
+    mult = 1.0 if scale is None or vectors[6] is not None else float(scale)
     h = codes = scales = None
     kind = 0
     if out == "float32":
@@ -518,16 +519,15 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
         raise KernelError(f"norm_residual_norm: h is float32, bfloat16 or \"mx4\", not {out}")
     if next_weight is not None:
         if out == "mx4":
-            h = Mx4._new(n, dm, at, False)
-            codes, scales, kind = h.codes, h.scales, 4
+            h = Mx4._new(n, dm, x, False)
+            codes, scales, kind = h._at_codes, h._at_scales, 4
         else:
-            h = codes = torch.empty((n, dm), dtype=out, device=at)
-            kind = _DT[out]
+            h = x.new_empty((n, dm), dtype=out)
+            codes, kind = h.data_ptr(), _DT[out]
     _check(lib().jb_norm_residual_norm(
-        _p(x), _p(y), y.shape[0], n * dm, _p(y_bias), _p(y_gate), Sg, n * g_ld, g_ld, gate_col0, _p(gate_bias),
-        _p(post_weight), _p(post_bias), float(eps), _p(scale), mult, _p(next_weight), _p(next_bias),
-        float(eps if next_eps is None else next_eps), 1 if rms else 0, _p(codes), _p(scales), kind, n, dm, _stream()),
-        "norm_residual_norm", 1 if n else 0)
+        x.data_ptr(), y.data_ptr(), S, n * dm, vectors[0], gate, Sg, n * g_ld, g_ld, gate_col0, vectors[1], vectors[2],
+        vectors[3], eps, vectors[6], mult, vectors[4], vectors[5], eps if next_eps is None else next_eps, rms, codes, scales,
+        kind, n, dm, _stream()), "norm_residual_norm", 1 if n else 0)
     return h
 
 
@@ -1329,10 +1329,10 @@ class Mx4:
     ``codes``: uint8 [rows, 16 ceil(k / 32)], value 2i of a row in the low half of byte i;
     ``scales``: uint8 [ceil(rows / 128), ceil(k / 256), 1024], for each 128 rows and 256 of k the
     exponents + 127 of the blocks of 32 values (255: the block stands for NaNs), block b of row r
-    at 512 (b / 4) + 16 (r % 32) + 4 (r / 32 % 4) + b % 4.  Bytes of rows past the last one are
-    not written and not used."""
+    at 512 (b / 4 % 2) + 16 (r % 32) + 4 (r / 32 % 4) + b % 4 of chunk b / 8.  Bytes of rows past the
+    last one are not written and not used; those of blocks past a row's end are zero."""
 
-    __slots__ = ("codes", "scales", "rows", "k", "settled")
+    __slots__ = ("rows", "k", "settled", "_buf", "_codes", "_scales", "_at_codes", "_at_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int):
         if k < 1 or rows < 0:
@@ -1341,23 +1341,48 @@ class Mx4:
         _need(scales, "scales", torch.uint8, ((rows + 127) // 128, (k + 255) // 256, 1024))
         if codes.data_ptr() % 16 or scales.data_ptr() % 16 or codes.device != scales.device:
             raise KernelError("Mx4: codes and scales must lie on one device at addresses that 16 divides")
-        self.codes, self.scales, self.rows, self.k = codes, scales, rows, k
+        self.rows, self.k = rows, k
         # whether no kernel that may start before the writer's end can follow the writer
         self.settled = True
+        self._buf = self._codes = codes
+        self._scales = scales
+        self._at_codes, self._at_scales = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _new(cls, rows: int, k: int, like: torch.Tensor, settled: bool) -> "Mx4":
+        """One allocation for both, codes first, on ``like``'s device."""
+        if k < 1:
+            raise KernelError("Mx4: rows of at least one value are needed")
+        self = object.__new__(cls)
+        n_codes = rows * ((k + 31) // 32 * 16)
+        self._buf = like.new_empty(n_codes + (rows + 127) // 128 * ((k + 255) // 256) * 1024, dtype=torch.uint8)
+        self._codes = self._scales = None
+        self._at_codes = self._buf.data_ptr()
+        self._at_scales = self._at_codes + n_codes
+        self.rows, self.k, self.settled = rows, k, settled
+        return self
 
     @property
     def shape(self) -> Tuple[int, int]:
         return (self.rows, self.k)
 
-    @classmethod
-    def _new(cls, rows: int, k: int, device: torch.device, settled: bool) -> "Mx4":
-        if k < 1:
-            raise KernelError("Mx4: rows of at least one value are needed")
-        self = object.__new__(cls)
-        self.codes = torch.empty((rows, (k + 31) // 32 * 16), dtype=torch.uint8, device=device)
-        self.scales = torch.empty(((rows + 127) // 128, (k + 255) // 256, 1024), dtype=torch.uint8, device=device)
-        self.rows, self.k, self.settled = rows, k, settled
-        return self
+    @property
+    def device(self) -> torch.device:
+        return self._buf.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            row = (self.k + 31) // 32 * 16
+            self._codes = self._buf[:self.rows * row].view(self.rows, row)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            at = self.rows * ((self.k + 31) // 32 * 16)
+            self._scales = self._buf[at:].view((self.rows + 127) // 128, (self.k + 255) // 256, 1024)
+        return self._scales
 
 
 def _here(t: torch.Tensor, name: str) -> None:
@@ -1373,8 +1398,8 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     _need(x, "x", _FLOATS, (None, None))
     _here(x, "x")
     n, k = x.shape
-    q = Mx4._new(n, k, x.device, True)
-    _check(lib().jb_mx4_quantize(_p(x), _DT[x.dtype], _p(q.codes), _p(q.scales), n, k, 0, _stream()), "mx4_quantize",
+    q = Mx4._new(n, k, x, True)
+    _check(lib().jb_mx4_quantize(x.data_ptr(), _DT[x.dtype], q._at_codes, q._at_scales, n, k, 0, _stream()), "mx4_quantize",
            1 if n else 0)
     return q
 
@@ -1387,19 +1412,19 @@ def mx4_gated_unit(gate_up: torch.Tensor, alpha: float = 1.0, limit: float = 0.0
     S, n, two_ff = gate_up.shape
     if two_ff % 2 or not S:
         raise KernelError("mx4_gated_unit: the gate_up width must be even, and at least one sum is needed")
-    q = Mx4._new(n, two_ff // 2, gate_up.device, False)
-    _check(lib().jb_mx4_gated_unit(_p(gate_up), S, n * two_ff, _p(q.codes), _p(q.scales), n, two_ff // 2, float(alpha),
-                                   float(limit), float(shift), _stream()), "mx4_gated_unit", 1 if n else 0)
+    q = Mx4._new(n, two_ff // 2, gate_up, False)
+    _check(lib().jb_mx4_gated_unit(gate_up.data_ptr(), S, n * two_ff, q._at_codes, q._at_scales, n, two_ff // 2, alpha, limit,
+                                   shift, _stream()), "mx4_gated_unit", 1 if n else 0)
     return q
 
 
 def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """What q stands for, as [rows, k] in float32 or bfloat16 (both hold every value exactly)."""
-    _here(q.codes, "q")
+    _here(q._buf, "q")
     if out_dtype not in _FLOATS:
         raise KernelError(f"mx4_values: the output is float32 or bfloat16, not {out_dtype}")
-    out = torch.empty((q.rows, q.k), dtype=out_dtype, device=q.codes.device)
-    _check(lib().jb_mx4_values(_p(q.codes), _p(q.scales), _p(out), _DT[out_dtype], q.rows, q.k, _stream()), "mx4_values",
+    out = q._buf.new_empty((q.rows, q.k), dtype=out_dtype)
+    _check(lib().jb_mx4_values(q._at_codes, q._at_scales, out.data_ptr(), _DT[out_dtype], q.rows, q.k, _stream()), "mx4_values",
            1 if q.rows else 0)
     return out
 
@@ -1407,28 +1432,32 @@ def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
 def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """a [n, k] . w [m, k]^T with both in microscaled 4-bit floats, summed in float32: [n, m] in float32 or
     bfloat16, the result itself and no stack of parts.  ``a``: an Mx4, or float32 or bfloat16 rows, which are
-    brought to 4 bits first, as mx4_quantize does."""
-    if not isinstance(w, Mx4):
+    brought to 4 bits on the way, as mx4_quantize does."""
+    if w.__class__ is not Mx4:
         raise KernelError("linear_mx4: the weight is an Mx4 (see mx4_quantize)")
     if out_dtype not in _FLOATS:
         raise KernelError(f"linear_mx4: the output is float32 or bfloat16, not {out_dtype}")
-    if not isinstance(a, Mx4):
-        _need(a, "activations", _FLOATS, (None, w.k))
-        _here(a, "activations")
-        n = a.shape[0]
-        q = Mx4._new(n, w.k, a.device, False)
-        _check(lib().jb_mx4_quantize(_p(a), _DT[a.dtype], _p(q.codes), _p(q.scales), n, w.k, 1, _stream()),
-               "linear_mx4", 1 if n else 0)
-        a = q
-    elif a.k != w.k:
-        raise KernelError(f"linear_mx4: rows of {a.k} values and a weight of {w.k}")
-    else:
-        _here(a.codes, "activations")
-    _here(w.codes, "weight")
-    n, m = a.rows, w.rows
-    out = torch.empty((n, m), dtype=out_dtype, device=w.codes.device)
-    _check(lib().jb_linear_mx4(_p(a.codes), _p(a.scales), _p(w.codes), _p(w.scales), _p(out), _DT[out_dtype], n, m, w.k,
-                               1 if w.settled else 0, _stream()), "linear_mx4", 1 if n and m else 0)
+    m, k = w.rows, w.k
+    _here(w._buf, "weight")
+    L = lib()
+    if a.__class__ is Mx4:
+        if a.k != k:
+            raise KernelError(f"linear_mx4: rows of {a.k} values and a weight of {k}")
+        _here(a._buf, "activations")
+        n = a.rows
+        out = w._buf.new_empty((n, m), dtype=out_dtype)
+        _check(L.jb_linear_mx4(a._at_codes, a._at_scales, w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k,
+                               w.settled, _stream()), "linear_mx4", 1 if n and m else 0)
+        return out
+    _need(a, "activations", _FLOATS, (None, k))
+    _here(a, "activations")
+    n = a.shape[0]
+    out = a.new_empty((n, m), dtype=out_dtype)
+    few = n <= L.jb_linear_mx4_rows_most()
+    scratch = None if few or not m else Mx4._new(n, k, a, False)
+    _check(L.jb_linear_mx4_rows(a.data_ptr(), _DT[a.dtype], None if scratch is None else scratch._at_codes, w._at_codes,
+                                w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k, w.settled, _stream()), "linear_mx4",
+           (1 if few else 2) if n and m else 0)
     return out
 
 
