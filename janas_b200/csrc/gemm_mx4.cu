@@ -259,11 +259,11 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                         ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / STAGES) & 1) ^ 1, abort, &g_gemm_mx4_error, 5));
                     uint8_t *stage = smem + s * Cfg::STAGE_BYTES + MX_W_BYTES;
                     if (ok && r < rows) {
-                        uint32_t word;
-                        const uint32_t packed = mx4_pack_chunk(v[d], word);
+                        uint32_t code;
+                        const uint32_t packed = mx4_pack_chunk(v[d], code);
                         *reinterpret_cast<uint32_t *>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = packed;
-                        if ((lane & 15) == 0)
-                            *reinterpret_cast<uint32_t *>(stage + Cfg::A_BYTES + MX4_TILE + (lane >> 4) * 512 + r * 16) = word;
+                        if ((lane & 3) == 0)
+                            stage[Cfg::A_BYTES + MX4_TILE + (lane >> 4) * 512 + r * 16 + ((lane >> 2) & 3)] = (uint8_t)code;
                     }
                     fetch(t + AHEAD, v[d]);
                     if (ok && g == groups - 1) {

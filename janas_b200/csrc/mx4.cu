@@ -14,11 +14,25 @@ namespace jb {
 template <typename T, bool VEC> struct RowSource {
     const T *x;
     int k;
-    __device__ __forceinline__ void load(size_t r, int col0, float *v) const
+    struct Values {
+        float v[8];
+    };
+    __device__ __forceinline__ void load(size_t r, int col0, Values &t) const
     {
-        load8<T, VEC>(x + r * (size_t)k + col0, k - col0, v);
+        load8<T, VEC>(x + r * (size_t)k + col0, k - col0, t.v);
     }
-    __device__ __forceinline__ void finish(float *) const {}
+    __device__ __forceinline__ uint32_t pack(Values &t, uint32_t &code) const { return mx4_pack_chunk(t.v, code); }
+};
+
+template <> struct RowSource<bf16, true> {
+    const bf16 *x;
+    int k;
+    typedef uint4 Values;
+    __device__ __forceinline__ void load(size_t r, int col0, Values &t) const
+    {
+        t = col0 < k ? *reinterpret_cast<const uint4 *>(x + r * (size_t)k + col0) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ uint32_t pack(Values &t, uint32_t &code) const { return mx4_pack_chunk(t, code); }
 };
 
 // The gated unit of the sums [S, n, 2 k]: columns [0, k) the gate, [k, 2 k) the up side.
@@ -28,8 +42,12 @@ template <bool VEC> struct UnitSource {
     size_t stride;
     int k;
     GatedUnit unit;
-    __device__ __forceinline__ void load(size_t r, int col0, float *v) const
+    struct Values {
+        float v[16];
+    };
+    __device__ __forceinline__ void load(size_t r, int col0, Values &to) const
     {
+        float *v = to.v;
         const float *g = z + r * 2 * (size_t)k + col0, *u = g + k;
         load8<float, VEC>(g, k - col0, v);
         load8<float, VEC>(u, k - col0, v + 8);
@@ -42,38 +60,48 @@ template <bool VEC> struct UnitSource {
                 v[i] += t[i];
         }
     }
-    __device__ __forceinline__ void finish(float *v) const
+    __device__ __forceinline__ uint32_t pack(Values &t, uint32_t &code) const
     {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            v[i] = gated_unit(v[i], v[8 + i], unit);
+            t.v[i] = gated_unit(t.v[i], t.v[8 + i], unit);
+        return mx4_pack_chunk(t.v, code);
     }
 };
 
-// Every warp takes U chunks that follow one another, all read before the first is packed: what is in flight decides the
-// bandwidth, and few rows are better spread over many warps (U = 1).  `total`: n times the chunks of a row.
-template <typename Source, int U, int VALUES>
+// A warp takes U chunks that follow one another at a time, all read before the first is packed.  `total`: n times the
+// chunks of a row.
+template <typename Source, int U>
 __global__ void __launch_bounds__(256)
 mx4_quantize_kernel(const Source src, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, unsigned total, int k, int early)
 {
     if (early)
         pdl_trigger();
     pdl_wait();
-    const unsigned chunks = mx4_chunks(k), first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * U;
-    float v[U][VALUES];
+    const unsigned chunks = mx4_chunks(k), step = gridDim.x * (blockDim.x >> 5) * U;
+    for (unsigned first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * U; first < total;) {
+        typename Source::Values v[U];
+        unsigned r = first / chunks, c = first - r * chunks, r0 = r, q0 = c;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const unsigned i = first + u, r = i / chunks;
-        if (i < total)
-            src.load(r, (i - r * chunks) * MX4_CHUNK + 8 * (threadIdx.x & 31), v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const unsigned i = first + u, r = i / chunks;
-        if (i < total) {
-            src.finish(v[u]);
-            mx4_store_chunk(v[u], r, i - r * chunks, k, codes, scales);
+        for (int u = 0; u < U; u++) {
+            if (first + u < total)
+                src.load(r, c * MX4_CHUNK + 8 * (threadIdx.x & 31), v[u]);
+            if (++c == chunks)
+                c = 0, r++;
         }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (first + u < total) {
+                uint32_t code;
+                const uint32_t packed = src.pack(v[u], code);
+                mx4_store_chunk(packed, code, r0, q0, k, codes, scales);
+            }
+            if (++q0 == chunks)
+                q0 = 0, r0++;
+        }
+        if (total - first <= step)
+            break;
+        first += step;
     }
     if (!early)
         __threadfence();
@@ -124,15 +152,16 @@ mx4_values_kernel(const uint8_t *codes, const uint8_t *scales, T *__restrict__ o
 static int mx4_unroll(size_t total) { return total >= (size_t)sm_count() * 32 * 4 ? 4 : 1; }
 static unsigned mx4_grid(size_t total, int unroll) { return (unsigned)((total + 8 * unroll - 1) / (8 * unroll)); }
 
-template <typename Source, int VALUES>
+template <typename Source, int U>
 static int quantize(const Source &src, void *codes, void *scales, int n, int k, int early, cudaStream_t st)
 {
     const size_t total = (size_t)n * mx4_chunks(k);
     if (total > 0xffffff00u)
         return JB_EINVAL;
-    const int u = mx4_unroll(total);
-    launch(u == 4 ? mx4_quantize_kernel<Source, 4, VALUES> : mx4_quantize_kernel<Source, 1, VALUES>, mx4_grid(total, u), 256, 0,
-           st, src, (uint8_t *)codes, (uint8_t *)scales, (unsigned)total, k, early);
+    const int u = mx4_unroll(total) > 1 ? U : 1;
+    const unsigned most = (unsigned)sm_count() * 8, grid = mx4_grid(total, u);
+    launch(u > 1 ? mx4_quantize_kernel<Source, U> : mx4_quantize_kernel<Source, 1>, grid < most ? grid : most, 256, 0, st, src,
+           (uint8_t *)codes, (uint8_t *)scales, (unsigned)total, k, early);
     return launch_status();
 }
 
@@ -172,7 +201,7 @@ extern "C" int jb_mx4_quantize(const void *x, int dt, void *codes, void *scales,
     if (n == 0)
         return JB_OK;
     const bool vec = k % 8 == 0 && (uintptr_t)x % 16 == 0;
-#define JB_Q(T, V) quantize<RowSource<T, V>, 8>(RowSource<T, V>{(const T *)x, k}, codes, scales, n, k, early, st)
+#define JB_Q(T, V) quantize<RowSource<T, V>, 4>(RowSource<T, V>{(const T *)x, k}, codes, scales, n, k, early, st)
     if (dt == 1)
         return vec ? JB_Q(bf16, true) : JB_Q(bf16, false);
     return vec ? JB_Q(float, true) : JB_Q(float, false);
@@ -189,8 +218,8 @@ extern "C" int jb_mx4_gated_unit(const float *z, int S, long long stride, void *
         return JB_OK;
     const GatedUnit unit{alpha, limit, shift};
     if (ff % 8 == 0 && (uintptr_t)z % 16 == 0 && stride % 4 == 0)
-        return quantize<UnitSource<true>, 16>(UnitSource<true>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
-    return quantize<UnitSource<false>, 16>(UnitSource<false>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
+        return quantize<UnitSource<true>, 2>(UnitSource<true>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
+    return quantize<UnitSource<false>, 2>(UnitSource<false>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
 }
 
 // What codes and scales stand for, as [n, k].

@@ -47,8 +47,8 @@ __device__ __forceinline__ float mx4_scale(uint32_t code)
     return __uint_as_float(code == 255u ? 0x7fffffffu : code == 0u ? 0x00400000u : code << 23);
 }
 
-// Eight values times inv, rounded to 4 bits: value i in bits 4 i.
-__device__ __forceinline__ uint32_t mx4_pack8(const float *v, float inv)
+// Eight values rounded to 4 bits: value i in bits 4 i.
+__device__ __forceinline__ uint32_t mx4_pack8(const float *v)
 {
     uint32_t r;
     asm("{\n\t"
@@ -60,19 +60,35 @@ __device__ __forceinline__ uint32_t mx4_pack8(const float *v, float inv)
         "mov.b32 %0, {a, b, c, d};\n\t"
         "}\n"
         : "=r"(r)
-        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
-          "f"(v[6] * inv), "f"(v[7] * inv));
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
-
-// The bits of the largest magnitude among eight values (a NaN is larger than an infinity).
-__device__ __forceinline__ uint32_t mx4_top8(const float *v)
+// The same of the values times inv, a power of two.
+__device__ __forceinline__ uint32_t mx4_pack8(const float *v, float inv)
 {
-    uint32_t t = 0;
+    float t[8];
 #pragma unroll
     for (int i = 0; i < 8; i++)
-        t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
-    return t;
+        t[i] = v[i] * inv;
+    return mx4_pack8(t);
+}
+
+// The larger of two magnitudes; a NaN is larger than all.
+__device__ __forceinline__ float mx4_larger(float a, float b)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
+// The bits of the largest magnitude among eight values.
+__device__ __forceinline__ uint32_t mx4_top8(const float *v)
+{
+    float t = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; i++)
+        t = mx4_larger(t, fabsf(v[i]));
+    return __float_as_uint(t);
 }
 
 // Eight consecutive floats of which `left` exist; zeros for the others.  VEC: all eight or none, at a 16-byte boundary.
@@ -101,33 +117,70 @@ template <typename T, bool VEC> __device__ __forceinline__ void load8(const T *p
     }
 }
 
-// A warp packs a chunk of 256 values, eight to a lane (zeros past the row's end): the lane's codes, and in lanes 0 and 16
-// the scales' codes of the four blocks of their half of the chunk.
-__device__ __forceinline__ uint32_t mx4_pack_chunk(const float *v, uint32_t &word)
+// A warp packs a chunk of 256 values, eight to a lane (zeros past the row's end): the lane's codes, and its block's scale's
+// code, which the four lanes of a block share.
+__device__ __forceinline__ uint32_t mx4_pack_chunk(const float *v, uint32_t &code)
 {
     uint32_t top = mx4_top8(v);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t code = mx4_scale_code(top);
-    word = code;
-    word |= __shfl_down_sync(0xffffffffu, code, 4) << 8;
-    word |= __shfl_down_sync(0xffffffffu, code, 8) << 16;
-    word |= __shfl_down_sync(0xffffffffu, code, 12) << 24;
+    code = mx4_scale_code(top);
     return mx4_pack8(v, mx4_inverse(code));
 }
 
-// The same, to memory: chunk c of row r.
-__device__ __forceinline__ void mx4_store_chunk(const float *v, size_t r, int c, int k, uint8_t *__restrict__ codes,
-                                                uint8_t *__restrict__ scales)
+// The same for eight bfloat16 as they lie in memory: magnitudes and the products with a power of two two at a time.
+__device__ __forceinline__ uint32_t mx4_pack_chunk(const uint4 &x, uint32_t &code)
+{
+    uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = max(top & 0xffff0000u, top << 16);
+    code = mx4_scale_code(top);
+    const uint32_t inv = (254u - min(code, 252u)) * 0x00800080u;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t p;
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(p) : "r"(w[i]), "r"(inv));
+        v[2 * i] = __uint_as_float(p << 16);
+        v[2 * i + 1] = __uint_as_float(p & 0xffff0000u);
+    }
+    return mx4_pack8(v);
+}
+
+// A lane's four values of a block that eight lanes share, in 16 bits, and the block's scale's code.
+__device__ __forceinline__ uint32_t mx4_pack4(const float4 &x, uint32_t &code)
+{
+    float t = mx4_larger(mx4_larger(fabsf(x.x), fabsf(x.y)), mx4_larger(fabsf(x.z), fabsf(x.w)));
+    uint32_t top = __float_as_uint(t);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+    code = mx4_scale_code(top);
+    const float inv = mx4_inverse(code);
+    uint32_t r;
+    asm("{\n\t"
+        ".reg .b8 a, b;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "mov.b32 %0, {a, b, a, b};\n\t"
+        "}\n"
+        : "=r"(r)
+        : "f"(x.x * inv), "f"(x.y * inv), "f"(x.z * inv), "f"(x.w * inv));
+    return r;
+}
+
+// Packed values to memory: chunk c of row r.
+__device__ __forceinline__ void mx4_store_chunk(uint32_t packed, uint32_t code, size_t r, int c, int k,
+                                                uint8_t *__restrict__ codes, uint8_t *__restrict__ scales)
 {
     const int lane = threadIdx.x & 31;
-    uint32_t word;
-    const uint32_t packed = mx4_pack_chunk(v, word);
     const size_t row_bytes = mx4_row_bytes(k), at = (size_t)c * (MX4_CHUNK / 2) + lane * 4;
     if (at < row_bytes)
         *reinterpret_cast<uint32_t *>(codes + r * row_bytes + at) = packed;
-    if ((lane & 15) == 0)
-        *reinterpret_cast<uint32_t *>(scales + mx4_scale_at(r, c, mx4_chunks(k), lane >> 4)) = word;
+    if ((lane & 3) == 0)
+        scales[mx4_scale_at(r, c, mx4_chunks(k), lane >> 4) + ((lane >> 2) & 3)] = (uint8_t)code;
 }
 
 // The numbers that the 8 codes of a word stand for.

@@ -479,22 +479,22 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
     a weight and optionally a bias (float32 [dm]); post_weight None: N1(u) = u; next_weight None: no h, None is
     returned.  h is [n, dm] in ``out``: torch.float32, torch.bfloat16, or "mx4" for an Mx4."""
     _need(x, "x", torch.float32, (None, None))
-    _here(x, "x")
+    st = _stream_of(x, "x")
     n, dm = x.shape
     y = stack(y)
     _need(y, "y", torch.float32, (None, n, dm))
     here = x.get_device()
-    vectors, vec = [], (dm,)
-    for t, name in ((y_bias, "y_bias"), (gate_bias, "gate_bias"), (post_weight, "post_weight"), (post_bias, "post_bias"),
-                    (next_weight, "next_weight"), (next_bias, "next_bias"),
-                    (scale if scale.__class__ is not float else None, "scale")):
-        if t is None or t.__class__ is int:
-            vectors.append(None)
-            continue
-        _need(t, name, torch.float32, vec)
-        if t.get_device() != here:
-            raise KernelError(f"{name}: on another device than x")
-        vectors.append(t.data_ptr())
+    yb = None if y_bias is None else _vector(y_bias, "y_bias", dm, here)
+    gb = None if gate_bias is None else _vector(gate_bias, "gate_bias", dm, here)
+    w1 = None if post_weight is None else _vector(post_weight, "post_weight", dm, here)
+    b1 = None if post_bias is None else _vector(post_bias, "post_bias", dm, here)
+    w2 = None if next_weight is None else _vector(next_weight, "next_weight", dm, here)
+    b2 = None if next_bias is None else _vector(next_bias, "next_bias", dm, here)
+    sc, mult = None, 1.0
+    if isinstance(scale, torch.Tensor):
+        sc = _vector(scale, "scale", dm, here)
+    elif scale is not None:
+        mult = float(scale)
     Sg, g_ld, gate = 0, 0, None
     if y_gate is not None:
         y_gate = stack(y_gate)
@@ -510,7 +510,6 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
     S = y.shape[0]
     if not S or y.get_device() != here:
         raise KernelError("norm_residual_norm: y needs at least one sum, on x's device")
-    mult = 1.0 if scale is None or vectors[6] is not None else float(scale)
     h = codes = scales = None
     kind = 0
     if out == "float32":
@@ -525,9 +524,8 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
             h = x.new_empty((n, dm), dtype=out)
             codes, kind = h.data_ptr(), _DT[out]
     _check(lib().jb_norm_residual_norm(
-        x.data_ptr(), y.data_ptr(), S, n * dm, vectors[0], gate, Sg, n * g_ld, g_ld, gate_col0, vectors[1], vectors[2],
-        vectors[3], eps, vectors[6], mult, vectors[4], vectors[5], eps if next_eps is None else next_eps, rms, codes, scales,
-        kind, n, dm, _stream()), "norm_residual_norm", 1 if n else 0)
+        x.data_ptr(), y.data_ptr(), S, n * dm, yb, gate, Sg, n * g_ld, g_ld, gate_col0, gb, w1, b1, eps, sc, mult, w2, b2,
+        eps if next_eps is None else next_eps, rms, codes, scales, kind, n, dm, st), "norm_residual_norm", 1 if n else 0)
     return h
 
 
@@ -1385,10 +1383,26 @@ class Mx4:
         return self._scales
 
 
-def _here(t: torch.Tensor, name: str) -> None:
-    """The launch goes to the current device's stream: a tensor of another device is refused."""
-    if t.get_device() != torch.cuda.current_device():
-        raise KernelError(f"{name}: on {t.device}, but the current device is {torch.cuda.current_device()}")
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _stream_of(t: torch.Tensor, name: str) -> int:
+    """The current stream's handle.  It belongs to the current device: a tensor of another one is refused."""
+    device = _current_device()
+    if t.get_device() != device:
+        raise KernelError(f"{name}: on {t.device}, but the current device is {device}")
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+def _vector(t: torch.Tensor, name: str, size: int, device: int) -> int:
+    """The address of a contiguous float32 vector [size] on the device."""
+    if (t.__class__ not in _TENSORS and not isinstance(t, torch.Tensor)) or t.get_device() != device \
+            or t.dtype is not torch.float32 or t.dim() != 1 or t.size(0) != size or not t.is_contiguous():
+        raise KernelError(f"{name}: a contiguous float32 vector of {size} values on x's device is needed")
+    return t.data_ptr()
+
+
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4:
@@ -1396,10 +1410,10 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     as 2^s times numbers of {0, 0.5, 1, 1.5, 2, 3, 4, 6} and a sign, s = floor(log2 max |x|) - 2 (at least
     -127), rounded to nearest, ties to even, at most 6.  A block with a NaN or an infinity stands for NaNs."""
     _need(x, "x", _FLOATS, (None, None))
-    _here(x, "x")
+    st = _stream_of(x, "x")
     n, k = x.shape
     q = Mx4._new(n, k, x, True)
-    _check(lib().jb_mx4_quantize(x.data_ptr(), _DT[x.dtype], q._at_codes, q._at_scales, n, k, 0, _stream()), "mx4_quantize",
+    _check(lib().jb_mx4_quantize(x.data_ptr(), _DT[x.dtype], q._at_codes, q._at_scales, n, k, 0, st), "mx4_quantize",
            1 if n else 0)
     return q
 
@@ -1408,23 +1422,23 @@ def mx4_gated_unit(gate_up: torch.Tensor, alpha: float = 1.0, limit: float = 0.0
     """``swiglu`` of a stack [S, n, 2 ff] with the result in microscaled 4-bit floats, [n, ff]."""
     gate_up = stack(gate_up)
     _need(gate_up, "gate_up", torch.float32, (None, None, None))
-    _here(gate_up, "gate_up")
+    st = _stream_of(gate_up, "gate_up")
     S, n, two_ff = gate_up.shape
     if two_ff % 2 or not S:
         raise KernelError("mx4_gated_unit: the gate_up width must be even, and at least one sum is needed")
     q = Mx4._new(n, two_ff // 2, gate_up, False)
     _check(lib().jb_mx4_gated_unit(gate_up.data_ptr(), S, n * two_ff, q._at_codes, q._at_scales, n, two_ff // 2, alpha, limit,
-                                   shift, _stream()), "mx4_gated_unit", 1 if n else 0)
+                                   shift, st), "mx4_gated_unit", 1 if n else 0)
     return q
 
 
 def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """What q stands for, as [rows, k] in float32 or bfloat16 (both hold every value exactly)."""
-    _here(q._buf, "q")
+    st = _stream_of(q._buf, "q")
     if out_dtype not in _FLOATS:
         raise KernelError(f"mx4_values: the output is float32 or bfloat16, not {out_dtype}")
     out = q._buf.new_empty((q.rows, q.k), dtype=out_dtype)
-    _check(lib().jb_mx4_values(q._at_codes, q._at_scales, out.data_ptr(), _DT[out_dtype], q.rows, q.k, _stream()), "mx4_values",
+    _check(lib().jb_mx4_values(q._at_codes, q._at_scales, out.data_ptr(), _DT[out_dtype], q.rows, q.k, st), "mx4_values",
            1 if q.rows else 0)
     return out
 
@@ -1438,25 +1452,27 @@ def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tenso
     if out_dtype not in _FLOATS:
         raise KernelError(f"linear_mx4: the output is float32 or bfloat16, not {out_dtype}")
     m, k = w.rows, w.k
-    _here(w._buf, "weight")
+    st = _stream_of(w._buf, "weight")
     L = lib()
     if a.__class__ is Mx4:
         if a.k != k:
             raise KernelError(f"linear_mx4: rows of {a.k} values and a weight of {k}")
-        _here(a._buf, "activations")
+        if a._buf.get_device() != w._buf.get_device():
+            raise KernelError("linear_mx4: the rows and the weight are on different devices")
         n = a.rows
         out = w._buf.new_empty((n, m), dtype=out_dtype)
         _check(L.jb_linear_mx4(a._at_codes, a._at_scales, w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k,
-                               w.settled, _stream()), "linear_mx4", 1 if n and m else 0)
+                               w.settled, st), "linear_mx4", 1 if n and m else 0)
         return out
     _need(a, "activations", _FLOATS, (None, k))
-    _here(a, "activations")
+    if a.get_device() != w._buf.get_device():
+        raise KernelError("linear_mx4: the rows and the weight are on different devices")
     n = a.shape[0]
     out = a.new_empty((n, m), dtype=out_dtype)
     few = n <= L.jb_linear_mx4_rows_most()
     scratch = None if few or not m else Mx4._new(n, k, a, False)
     _check(L.jb_linear_mx4_rows(a.data_ptr(), _DT[a.dtype], None if scratch is None else scratch._at_codes, w._at_codes,
-                                w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k, w.settled, _stream()), "linear_mx4",
+                                w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k, w.settled, st), "linear_mx4",
            (1 if few else 2) if n and m else 0)
     return out
 

@@ -5,10 +5,16 @@
 //   x <-  x + mult * scale * N1(u)                                    (N1 and the vector scale are optional)
 //   h  =  N2(x)                                                       (optional)
 //
+// Every product and sum is rounded by itself and the norms' factor is one reciprocal root, so that the steps one by one give
+// the same values up to their sums' order: what is left of a difference decides how often the 4-bit form of h falls on the
+// other side of a border.
+//
 // N: a layer norm (t - mean) / sqrt(var + eps) * w + b, var the mean of the squared deviations, or with `rms`
 // t / sqrt(mean(t^2) + eps) * w + b.  h is float32, bfloat16 or microscaled 4-bit floats (mx4.cuh).
 //
-// Bound by memory.  A block per row, which stays in shared memory between the passes.
+// Bound by memory, and by the chain of sums for few rows.  A block per row, which stays in registers between the sums, up to
+// four groups of four values a thread; rows that whole 16-byte loads do not fit, or longer ones, stay in shared memory.
+// How a row is shared out among the threads depends on its length alone, so its bits are the same in any batch.
 #include "kernels.h"
 #include "mx4.cuh"
 
@@ -26,17 +32,158 @@ struct NormsArgs {
     uint8_t *scales;
 };
 
+__device__ __forceinline__ float gated(float v, float z) { return __fmul_rn(v, 1.0f / (1.0f + expf(-z))); }
+// t inv w (+ b), and x + c t
+__device__ __forceinline__ float normed(float t, float inv, float w, const float *b)
+{
+    const float v = __fmul_rn(__fmul_rn(t, inv), w);
+    return b ? __fadd_rn(v, *b) : v;
+}
+__device__ __forceinline__ float added(float x, float c, float t) { return __fadd_rn(x, __fmul_rn(c, t)); }
+
 // mean (0 with rms) and 1 / sqrt(var + eps) of a row in shared memory
 __device__ __forceinline__ void row_moments(const float *row, int dm, float sum, bool rms, float eps, float *red,
                                             float &mean, float &inv)
 {
-    mean = rms ? 0.0f : block_sum(sum, red) / (float)dm;
+    mean = rms ? 0.0f : block_sum(sum, red) * (1.0f / dm);
     float sq = 0.0f;
     for (int i = threadIdx.x; i < dm; i += blockDim.x) {
         const float d = row[i] - mean;
         sq = fmaf(d, d, sq);
     }
-    inv = 1.0f / sqrtf(block_sum(sq, red) / (float)dm + eps);
+    inv = rsqrtf(block_sum(sq, red) * (1.0f / dm) + eps);
+}
+
+// The block's sum of v: every warp adds up all warps' sums from a slot that no other sum uses, so one barrier is enough.
+__device__ __forceinline__ float slot_sum(float v, float *slot)
+{
+    const int lane = threadIdx.x & 31;
+    v = warp_sum(v);
+    if (lane == 0)
+        slot[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_sum(lane < (int)(blockDim.x >> 5) ? slot[lane] : 0.0f);
+}
+
+__device__ __forceinline__ float sum4(const float4 &v) { return (v.x + v.y) + (v.z + v.w); }
+
+// The norm of a row in registers: t <- (t - mean) / sqrt(var + eps) * w + b.  Values past the row's end are zeros before
+// and whatever comes out after.
+template <int NV>
+__device__ __forceinline__ void norm_row(float4 *t, int dm, bool rms, float eps, const float *w, const float *b, float *slots)
+{
+    float mean = 0.0f;
+    if (!rms) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            sum += sum4(t[j]);
+        mean = slot_sum(sum, slots) * (1.0f / dm);
+    }
+    float sq = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        if (4 * (int)(threadIdx.x + j * blockDim.x) < dm) {
+            t[j].x -= mean, t[j].y -= mean, t[j].z -= mean, t[j].w -= mean;
+            sq += (t[j].x * t[j].x + t[j].y * t[j].y) + (t[j].z * t[j].z + t[j].w * t[j].w);
+        }
+    }
+    const float inv = rsqrtf(slot_sum(sq, slots + 32) * (1.0f / dm) + eps);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = 4 * (threadIdx.x + j * blockDim.x);
+        if (i < dm) {
+            const float4 u = load4(w + i);
+            t[j] = make_float4(normed(t[j].x, inv, u.x, nullptr), normed(t[j].y, inv, u.y, nullptr),
+                               normed(t[j].z, inv, u.z, nullptr), normed(t[j].w, inv, u.w, nullptr));
+            if (b) {
+                const float4 c = load4(b + i);
+                t[j] = make_float4(__fadd_rn(t[j].x, c.x), __fadd_rn(t[j].y, c.y), __fadd_rn(t[j].z, c.z), __fadd_rn(t[j].w, c.w));
+            }
+        }
+    }
+}
+
+// The sum of four columns over a stack, after a vector or nothing.
+__device__ __forceinline__ float4 sum_stack(const float *bias, const float *p, int S, size_t stride)
+{
+    float4 v = load4(p);
+    if (bias) {
+        const float4 c = load4(bias);
+        v.x += c.x, v.y += c.y, v.z += c.z, v.w += c.w;
+    }
+    for (int s = 1; s < S; s++) {
+        const float4 u = load4(p + s * stride);
+        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    return v;
+}
+
+// NV groups of four values a thread; every address at a 16-byte boundary.
+template <int NV>
+__global__ void __launch_bounds__(1024)
+sublayer_norms_vec_kernel(const NormsArgs a)
+{
+    __shared__ float slots[4][32];
+    pdl_trigger();
+    pdl_wait();
+    const size_t r = blockIdx.x;
+    const int dm = a.dm;
+    float *x = a.x + r * dm;
+    float4 t[NV], old[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = 4 * (threadIdx.x + j * blockDim.x);
+        t[j] = old[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < dm) {
+            old[j] = load4(x + i);
+            t[j] = sum_stack(a.y_bias ? a.y_bias + i : nullptr, a.y + r * dm + i, a.Sy, a.y_stride);
+            if (a.g) {
+                const float4 z = sum_stack(a.g_bias ? a.g_bias + i : nullptr, a.g + r * a.g_ld + a.g_col0 + i, a.Sg, a.g_stride);
+                t[j] = make_float4(gated(t[j].x, z.x), gated(t[j].y, z.y), gated(t[j].z, z.z), gated(t[j].w, z.w));
+            }
+        }
+    }
+    if (a.w1)
+        norm_row<NV>(t, dm, a.rms, a.eps1, a.w1, a.b1, slots[0]);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = 4 * (threadIdx.x + j * blockDim.x);
+        if (i < dm) {
+            const float4 c = a.scale ? load4(a.scale + i) : make_float4(1.f, 1.f, 1.f, 1.f);
+            t[j] = make_float4(added(old[j].x, a.mult * c.x, t[j].x), added(old[j].y, a.mult * c.y, t[j].y),
+                               added(old[j].z, a.mult * c.z, t[j].z), added(old[j].w, a.mult * c.w, t[j].w));
+            store4(x + i, t[j]);
+        }
+    }
+    if (!a.w2)
+        return;
+    norm_row<NV>(t, dm, a.rms, a.eps2, a.w2, a.b2, slots[2]);
+    const int blocks = (dm + 31) / 32, chunks = mx4_chunks(dm);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int g = threadIdx.x + j * blockDim.x, i = 4 * g;
+        if (a.out_kind == OUT_MX4) {
+            // eight lanes have a block; what lies past the row's end in its last one is zero
+            uint32_t code;
+            const uint32_t packed = mx4_pack4(i < dm ? t[j] : make_float4(0.f, 0.f, 0.f, 0.f), code);
+            if (g < 8 * blocks)
+                *reinterpret_cast<uint16_t *>((uint8_t *)a.out + r * mx4_row_bytes(dm) + 2 * g) = (uint16_t)packed;
+            const int b = g >> 3;
+            if ((g & 7) == 0 && b < blocks)
+                a.scales[mx4_scale_at(r, b >> 3, chunks, (b >> 2) & 1) + (b & 3)] = (uint8_t)code;
+        } else if (i < dm) {
+            if (a.out_kind == OUT_BF16)
+                store4((bf16 *)a.out + r * dm + i, t[j]);
+            else
+                store4((float *)a.out + r * dm + i, t[j]);
+        }
+    }
+    if (a.out_kind == OUT_MX4) {
+        const int b = blocks + threadIdx.x;         // the last chunk's blocks past the row's end
+        if (b < 8 * chunks)
+            a.scales[mx4_scale_at(r, b >> 3, chunks, (b >> 2) & 1) + (b & 3)] = 0;
+    }
 }
 
 __global__ void __launch_bounds__(256)
@@ -54,7 +201,7 @@ sublayer_norms_kernel(const NormsArgs a)
         float v = add_partials(a.y_bias ? a.y_bias[i] : 0.0f, a.y + r * dm + i, a.Sy, a.y_stride);
         if (a.g) {
             const float z = add_partials(a.g_bias ? a.g_bias[i] : 0.0f, a.g + r * a.g_ld + a.g_col0 + i, a.Sg, a.g_stride);
-            v = v / (1.0f + expf(-z));
+            v = gated(v, z);
         }
         row[i] = v;
         sum += v;
@@ -66,8 +213,8 @@ sublayer_norms_kernel(const NormsArgs a)
     for (int i = threadIdx.x; i < dm; i += blockDim.x) {
         float v = row[i];
         if (a.w1)
-            v = fmaf((v - mean) * inv, a.w1[i], a.b1 ? a.b1[i] : 0.0f);
-        v = fmaf(a.scale ? a.mult * a.scale[i] : a.mult, v, x[i]);
+            v = normed(v - mean, inv, a.w1[i], a.b1 ? a.b1 + i : nullptr);
+        v = added(x[i], a.scale ? a.mult * a.scale[i] : a.mult, v);
         x[i] = v;
         row[i] = v;
         sum += v;
@@ -83,14 +230,16 @@ sublayer_norms_kernel(const NormsArgs a)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int i = c * MX4_CHUNK + 8 * lane + j;
-                v[j] = i < dm ? fmaf((row[i] - mean) * inv, a.w2[i], a.b2 ? a.b2[i] : 0.0f) : 0.0f;
+                v[j] = i < dm ? normed(row[i] - mean, inv, a.w2[i], a.b2 ? a.b2 + i : nullptr) : 0.0f;
             }
-            mx4_store_chunk(v, r, c, dm, (uint8_t *)a.out, a.scales);
+            uint32_t code;
+            const uint32_t packed = mx4_pack_chunk(v, code);
+            mx4_store_chunk(packed, code, r, c, dm, (uint8_t *)a.out, a.scales);
         }
         return;
     }
     for (int i = threadIdx.x; i < dm; i += blockDim.x) {
-        const float v = fmaf((row[i] - mean) * inv, a.w2[i], a.b2 ? a.b2[i] : 0.0f);
+        const float v = normed(row[i] - mean, inv, a.w2[i], a.b2 ? a.b2 + i : nullptr);
         if (a.out_kind == OUT_BF16)
             ((bf16 *)a.out)[r * dm + i] = from_f<bf16>(v);
         else
@@ -117,11 +266,20 @@ extern "C" int jb_norm_residual_norm(float *x, const float *y, int Sy, long long
         (w2 && !out) || (out_kind != OUT_F32 && out_kind != OUT_BF16 && out_kind != OUT_MX4) ||
         (w2 && out_kind == OUT_MX4 && !out_scales))
         return JB_EINVAL;
+    NormsArgs a{x, y, y_bias, g, g_bias, w1, b1, scale, w2, b2, Sy, Sg, g_ld, g_col0, rms, out_kind, dm,
+                (size_t)y_stride, (size_t)g_stride, eps1, mult, eps2, out, (uint8_t *)out_scales};
+    const uintptr_t all = (uintptr_t)x | (uintptr_t)y | (uintptr_t)y_bias | (uintptr_t)g | (uintptr_t)g_bias | (uintptr_t)w1 |
+                          (uintptr_t)b1 | (uintptr_t)scale | (uintptr_t)w2 | (uintptr_t)b2 | (uintptr_t)out;
+    if (dm % 4 == 0 && dm <= 16384 && all % 16 == 0 && y_stride % 4 == 0 && (!g || (g_stride % 4 == 0 && g_ld % 4 == 0 && g_col0 % 4 == 0))) {
+        const int nv = dm <= 1024 ? 1 : dm <= 8192 ? 2 : 4;
+        const unsigned threads = (unsigned)((dm / 4 + nv * 32 - 1) / (nv * 32)) * 32;
+        launch(nv == 1 ? sublayer_norms_vec_kernel<1> : nv == 2 ? sublayer_norms_vec_kernel<2> : sublayer_norms_vec_kernel<4>,
+               (unsigned)n, threads, 0, st, a);
+        return launch_status();
+    }
     static unsigned long long allowed = 0;
     if (!allow_dynamic_smem(sublayer_norms_kernel, jb_norm_residual_norm_most() * 4, allowed))
         return JB_ELAUNCH;
-    NormsArgs a{x, y, y_bias, g, g_bias, w1, b1, scale, w2, b2, Sy, Sg, g_ld, g_col0, rms, out_kind, dm,
-                (size_t)y_stride, (size_t)g_stride, eps1, mult, eps2, out, (uint8_t *)out_scales};
     launch(sublayer_norms_kernel, (unsigned)n, 256, (size_t)dm * 4, st, a);
     return launch_status();
 }
