@@ -338,6 +338,262 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                      ::"r"(tmem), "r"((uint32_t)Cfg::TMEM_COLS) : "memory");
 }
 
+
+// ------------------------------------------------------------------ many rows
+// Pairs of CTAs (a cluster of two) that share their MMAs: 256 features by BN rows, each CTA with 128 of the features, half
+// of the rows' codes, the scales of its features and of all the rows.  A CTA brings in 35 KB for 128 x 256 outputs' 256
+// values of k instead of the 51 KB that it would need alone: what an SM can take in is what bounds the product.  The
+// leader's warp 1 issues for both; a stage's loads of both CTAs report to the leader's barrier.  One pair stays on its two
+// SMs for all its tiles; the epilogue's warps take the accumulator into registers at once, so the next tile's MMAs run
+// while they store.
+constexpr int MX_PAIR_M = 2 * MX_TILE_M;
+
+template <int BN> struct MxPairCfg {
+    static constexpr int A_BYTES = BN / 2 * (MX4_CHUNK / 2);
+    static constexpr int B_SCALES = (BN + 127) / 128 * MX4_TILE;
+    static constexpr int STAGE_BYTES = MX_W_BYTES + A_BYTES + MX4_TILE + B_SCALES;
+    static constexpr int STAGES = 222 * 1024 / STAGE_BYTES > 8 ? 8 : 222 * 1024 / STAGE_BYTES;
+    static constexpr int SLOT_COLS = 8 + B_SCALES / 128;    // columns of a stage's scales
+    static_assert(BN + STAGES * SLOT_COLS <= 512, "tensor memory");
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */;
+};
+
+// A tiled load whose bytes are counted at a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+// The MMAs so far report to the barrier at the same place of both CTAs.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t"
+        "}\n"
+        ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t mine, uint32_t rank)
+{
+    uint32_t ra;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(mine), "r"(rank));
+    return ra;
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Copies 512 bytes of scales (32 rows of 16) to four columns of tensor memory, in both CTAs of the pair.
+__device__ __forceinline__ void mx_scales_pair(uint32_t col, uint32_t smem_addr)
+{
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(col), "l"(mx_scale_desc(smem_addr)) : "memory");
+}
+
+__device__ __forceinline__ void mx_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                            uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}\n"
+        : "=r"(ok));
+    return ok != 0;
+}
+
+template <int BN, typename TO>
+__global__ void __launch_bounds__(MX_THREADS, 1)
+gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                     const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_as,
+                     TO *__restrict__ out, int n, int m, int chunks, int tiles_n, int tiles, int w_early)
+{
+    using Cfg = MxPairCfg<BN>;
+    constexpr int STAGES = Cfg::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = (uint64_t *)(smem + STAGES * Cfg::STAGE_BYTES);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 2);
+    volatile int *abort = (volatile int *)(tmem_slot + 1);
+
+    const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES),
+                   drained = smem_u32(bars + 2 * STAGES + 1);
+    if (threadIdx.x == 0) {
+        prefetch_tensor_map(&map_w);
+        prefetch_tensor_map(&map_a);
+        prefetch_tensor_map(&map_ws);
+        prefetch_tensor_map(&map_as);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(accum, 1);
+        mbar_init(drained, 16);             // the epilogue's warps of both CTAs
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem = warp_uniform(*tmem_slot);
+    pdl_trigger();
+
+    if (warp == 0 && lane == 0) {
+        // ---------------------------------------------------------- loads
+        uint32_t it = 0;
+        const uint32_t lead_full = cluster_addr(full0, 0);
+        bool ok = true, waited = false;
+        if (!w_early) {
+            pdl_wait();
+            waited = true;
+        }
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int m0 = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M, n0 = tile % tiles_n * BN;
+            const int ws = (m0 >> 7) * chunks, as = (n0 >> 7) * chunks;
+            for (int c = 0; c < chunks; c++, it++) {
+                const int s = it % STAGES;
+                if (it >= STAGES && !mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, abort, &g_gemm_mx4_error, 1)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t dst = smem_u32(smem + s * Cfg::STAGE_BYTES), bar = lead_full + 8 * s;
+                if (rank == 0)
+                    mbar_expect_tx(full0 + 8 * s, 2 * Cfg::STAGE_BYTES);
+                tma_load_pair(dst, &map_w, bar, c * (MX4_CHUNK / 2), m0);
+                tma_load_pair(dst + MX_W_BYTES + Cfg::A_BYTES, &map_ws, bar, 0, ws + c);
+                if (!waited) {
+                    pdl_wait();
+                    waited = true;
+                }
+                tma_load_pair(dst + MX_W_BYTES, &map_a, bar, c * (MX4_CHUNK / 2), n0 + (int)rank * (BN / 2));
+#pragma unroll
+                for (int t = 0; t < (BN + 127) / 128; t++)
+                    tma_load_pair(dst + MX_W_BYTES + Cfg::A_BYTES + MX4_TILE * (1 + t), &map_as, bar, 0, as + t * chunks + c);
+            }
+        }
+        if (*abort && rank == 0) {
+            // the loads in flight of both CTAs: wait for each stage's last use, once, with the limit (the other CTA then
+            // waits for this one at the cluster's barrier)
+            volatile int never = 0;
+            for (uint32_t u = it > STAGES ? it - STAGES : 0; u < it; u++)
+                mbar_wait(full0 + 8 * (u % STAGES), (u / STAGES) & 1, &never, &g_gemm_mx4_error, 4);
+        }
+    } else if (warp == 1 && rank == 0) {
+        // --------------------------------------------------------------- MMAs of both CTAs
+        constexpr uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(MX_PAIR_M >> 4) << 24);
+        constexpr uint32_t idesc2 = idesc | (2u << 4) | (2u << 29);
+        const bool issue = elect_one();
+        uint32_t it = 0, done = 0;
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += pairs, done++) {
+            if (done && !__all_sync(0xffffffffu, mbar_wait(drained, (done - 1) & 1, abort, &g_gemm_mx4_error, 6)))
+                break;
+            tc_fence_after();
+            for (int c = 0; c < chunks; c++, it++) {
+                const int s = it % STAGES;
+                if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (it / STAGES) & 1, abort, &g_gemm_mx4_error, 2))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t base = smem_u32(smem) + s * Cfg::STAGE_BYTES, sc = base + MX_W_BYTES + Cfg::A_BYTES;
+                const uint32_t ca = tmem + BN + s * Cfg::SLOT_COLS, cb = ca + 8;
+                if (issue) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        mx_scales_pair(ca + 4 * h, sc + 512 * h);
+#pragma unroll
+                        for (int t = 0; t < (BN + 127) / 128; t++)      // a half's columns of all the rows side by side
+                            mx_scales_pair(cb + (BN + 127) / 128 * 4 * h + 4 * t, sc + MX4_TILE * (1 + t) + 512 * h);
+                    }
+                    const uint64_t da = smem_desc_sw128(base, 16, 1024), db = smem_desc_sw128(base + MX_W_BYTES, 16, 1024);
+#pragma unroll
+                    for (int h = 0; h < 4; h++)
+                        mx_mma_pair(tmem, da + 2 * h, db + 2 * h, h & 1 ? idesc2 : idesc, ca + 4 * (h >> 1),
+                                    cb + (BN + 127) / 128 * 4 * (h >> 1), c != 0 || h != 0);
+                }
+                __syncwarp();
+                tc_commit_pair(empty0 + 8 * s);
+            }
+            tc_commit_pair(accum);
+        }
+    } else if (warp >= 2) {
+        // ------------------------------------------------------------ epilogue
+        constexpr int PART = BN / 2;
+        const int q = warp & 3, part = (warp - 2) >> 2;
+        const uint32_t lead_drained = cluster_addr(drained, 0);
+        uint32_t done = 0;
+        pdl_wait();
+        for (int tile = pair; tile < tiles; tile += pairs, done++) {
+            if (!__all_sync(0xffffffffu, mbar_wait(accum, done & 1, abort, &g_gemm_mx4_error, 3)))
+                break;
+            tc_fence_after();
+            const int f = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M + q * 32 + lane, r0 = tile % tiles_n * BN + part * PART;
+            uint32_t v[PART];
+#pragma unroll
+            for (int c = 0; c < PART; c += 32)
+                tc_ld32_nowait(tmem + ((uint32_t)(q * 32) << 16) + part * PART + c, v + c);
+            tc_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive_cluster(lead_drained);
+            if (f < m) {
+                TO *o = out + (size_t)r0 * m + f;
+                if (r0 + PART <= n) {
+#pragma unroll
+                    for (int j = 0; j < PART; j++, o += m)
+                        *o = from_f<TO>(__uint_as_float(v[j]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < PART; j++, o += m)
+                        if (r0 + j < n)
+                            *o = from_f<TO>(__uint_as_float(v[j]));
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_arrive();
+    cluster_wait();                 // neither CTA ends, or gives its tensor memory back, while the other's MMAs may run
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
 // A matrix of codes in boxes of box_rows x 128 bytes with the 128-byte swizzle; what lies outside reads as zero.
 static bool mx_tensor_map(const void *codes, int rows, int k, int box_rows, CUtensorMap *out)
 {
@@ -350,6 +606,42 @@ static bool mx_tensor_map(const void *codes, int rows, int k, int box_rows, CUte
     return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Scales as rows of 1,024 bytes, a chunk of 128 of the matrix's rows each.
+static bool mx_scale_map(const void *scales, int rows, int k, CUtensorMap *out)
+{
+    EncodeTiled enc = tensor_map_encoder();
+    if (!enc)
+        return false;
+    cuuint64_t dims[2] = {MX4_TILE / 4, (cuuint64_t)((rows + 127) / 128) * mx4_chunks(k)};
+    cuuint64_t strides[1] = {MX4_TILE};
+    cuuint32_t box[2] = {MX4_TILE / 4, 1}, estr[2] = {1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(scales), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, typename TO>
+static int launch_mx_pair(const void *ac, const void *as, const void *wc, const void *ws, TO *out, int n, int m, int k,
+                          int w_early, cudaStream_t st)
+{
+    using Cfg = MxPairCfg<BN>;
+    CUtensorMap map_w, map_a, map_ws, map_as;
+    if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || !mx_tensor_map(ac, n, k, BN / 2, &map_a) ||
+        !mx_scale_map(ws, m, k, &map_ws) || !mx_scale_map(as, n, k, &map_as))
+        return JB_EINVAL;
+    auto kern = gemm_mx4_pair_kernel<BN, TO>;
+    static unsigned long long allowed = 0;
+    if (!allow_dynamic_smem(kern, Cfg::SMEM_BYTES, allowed))
+        return JB_ELAUNCH;
+    const long long tiles_n = (n + BN - 1) / BN, tiles = tiles_n * ((m + MX_PAIR_M - 1) / MX_PAIR_M);
+    if (tiles > 0x7fffffff)
+        return JB_EINVAL;
+    const long long pairs = sm_count() / 2;
+    launch_cluster(kern, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), MX_THREADS, Cfg::SMEM_BYTES, st, 2u, map_w, map_a,
+                   map_ws, map_as, out, n, m, mx4_chunks(k), (int)tiles_n, (int)tiles, w_early);
+    return launch_status();
 }
 
 // Parts of k (1, 2, 4 or 8) that a product's tiles are shared out in.
@@ -399,7 +691,11 @@ static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, c
         return launch_mx<32, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 64)
         return launch_mx<64, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    return launch_mx<128, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 128)
+        return launch_mx<128, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 256)
+        return launch_mx_pair<128, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+    return launch_mx_pair<256, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
 }
 
 static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, int out_dt, int n, int m, int k)
