@@ -340,31 +340,44 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
 
 // ------------------------------------------------------------------ many rows
-// Pairs of CTAs (a cluster of two) that share their MMAs: 256 features by BN rows, each CTA with 128 of the features, half
-// of the rows' codes, the scales of its features and of all the rows.  A CTA brings in 35 KB for 128 x 256 outputs' 256
-// values of k instead of the 51 KB that it would need alone: what an SM can take in is what bounds the product.  The
-// leader's warp 1 issues for both; a stage's loads of both CTAs report to the leader's barrier.  One pair stays on its two
-// SMs for all its tiles; the epilogue's warps take the accumulator into registers at once, so the next tile's MMAs run
-// while they store.
+// Pairs of CTAs (a cluster of two) that share their MMAs: 256 features by 256 rows, each CTA with 128 of the features, half
+// of the rows' codes, the scales of its features and of all the rows.  The leader's warp 1 issues for both; the loads of
+// both CTAs report to the leader's barriers.  A pair stays on its two SMs for all its tiles; the epilogue's warps take the
+// accumulator into registers at once, so the next tile's MMAs run while they store.  (Two accumulators leave no room in
+// tensor memory for scales; with 192 rows they would fit, but an MMA of 64 values of k takes 135 cycles whether it is of
+// 128, 192 or 256 rows: 2,048 rows x 18,944 x 2,560 52 us with tiles of 192.)
+//
+// What bounds it: the MMAs, with the loads close behind.  A copy of a chunk's scales costs a fifth of what a chunk's codes
+// do, however few its bytes, so one copy brings two chunks' scales.
 constexpr int MX_PAIR_M = 2 * MX_TILE_M;
+constexpr int MX_PAIR_N = 256;
+constexpr int MX_GROUP = 2;         // chunks whose scales are copied together
+constexpr int MX_GROUPS = 3;        // such copies in shared memory
+constexpr int MX_ROW_TILES = MX_PAIR_N / 128;
+constexpr int MX_PAIR_STAGES = 6;
+constexpr int MX_PAIR_A_BYTES = MX_PAIR_N / 2 * (MX4_CHUNK / 2);
+constexpr int MX_PAIR_STAGE_BYTES = MX_W_BYTES + MX_PAIR_A_BYTES;
+constexpr int MX_PAIR_SCALE_BYTES = MX_GROUP * (1 + MX_ROW_TILES) * MX4_TILE;
+constexpr int MX_SLOT_COLS = 8 + 8 * MX_ROW_TILES;      // columns of tensor memory of a stage's scales
+static_assert(MX_PAIR_N + MX_PAIR_STAGES * MX_SLOT_COLS <= 512, "tensor memory");
+constexpr int MX_PAIR_SMEM = MX_PAIR_STAGES * MX_PAIR_STAGE_BYTES + MX_GROUPS * MX_PAIR_SCALE_BYTES + 1024 /* alignment */ +
+                             256 /* barriers */;
 
-template <int BN> struct MxPairCfg {
-    static constexpr int A_BYTES = BN / 2 * (MX4_CHUNK / 2);
-    static constexpr int B_SCALES = (BN + 127) / 128 * MX4_TILE;
-    static constexpr int STAGE_BYTES = MX_W_BYTES + A_BYTES + MX4_TILE + B_SCALES;
-    static constexpr int STAGES = 222 * 1024 / STAGE_BYTES > 8 ? 8 : 222 * 1024 / STAGE_BYTES;
-    static constexpr int SLOT_COLS = 8 + B_SCALES / 128;    // columns of a stage's scales
-    static_assert(BN + STAGES * SLOT_COLS <= 512, "tensor memory");
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */;
-};
-
-// A tiled load whose bytes are counted at a barrier of either CTA of the pair.
+// Tiled loads whose bytes are counted at a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
 {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4}], [%2];"
         ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 
@@ -387,72 +400,99 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t mine, uint32_t rank)
     return ra;
 }
 
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar)
+// Arrives at a barrier of either CTA.  What it hands over is tensor memory, read and fenced by tcgen05's own means: an
+// arrival that also released this thread's stores to the cluster would wait for them (2,000 cycles, measured).
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Copies 512 bytes of scales (32 rows of 16) to four columns of tensor memory, in both CTAs of the pair.
-__device__ __forceinline__ void mx_scales_pair(uint32_t col, uint32_t smem_addr)
+// A chunk's scales to tensor memory of both CTAs, by a whole warp whose lanes agree on the arguments: from column sa on the
+// features' eight columns, behind them the rows', a half chunk's columns of both row tiles side by side.  sa_mem, sb_mem:
+// their descriptors, half chunks 512 bytes apart and row tiles MX_GROUP * 1,024.
+__device__ __forceinline__ void mx_scales_pair(uint32_t sa, uint64_t sa_mem, uint64_t sb_mem)
 {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(col), "l"(mx_scale_desc(smem_addr)) : "memory");
-}
-
-__device__ __forceinline__ void mx_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
-                                            uint32_t accumulate)
-{
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-        "}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ bool elect_one()
-{
-    uint32_t ok;
     asm volatile(
         "{\n\t"
         ".reg .pred q;\n\t"
+        ".reg .b64 m1, n1, n2, n3;\n\t"
+        ".reg .b32 t1, u0, u1, u2, u3;\n\t"
+        "add.u64 m1, %1, 32;\n\t"
+        "add.u64 n1, %2, 32;\n\t"
+        "add.u64 n2, %2, %3;\n\t"
+        "add.u64 n3, n2, 32;\n\t"
+        "add.u32 t1, %0, 4;\n\t"
+        "add.u32 u0, %0, 8;\n\t"            // row tile 0, first half of the chunk
+        "add.u32 u1, %0, 16;\n\t"           // and second
+        "add.u32 u2, %0, 12;\n\t"           // row tile 1
+        "add.u32 u3, %0, 20;\n\t"
         "elect.sync _|q, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t"
+        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t"
+        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [u0], %2;\n\t"
+        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [u2], n2;\n\t"
+        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [t1], m1;\n\t"
+        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [u1], n1;\n\t"
+        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [u3], n3;\n\t"
         "}\n"
-        : "=r"(ok));
-    return ok != 0;
+        ::"r"(sa), "l"(sa_mem), "l"(sb_mem), "n"(MX_GROUP * MX4_TILE / 16) : "memory");
 }
 
-template <int BN, typename TO>
+// A chunk's four MMAs of a pair, by a whole warp whose lanes agree on the arguments (see tc_mma4).
+__device__ __forceinline__ void mx_chunk_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t sa, uint32_t accumulate)
+{
+    constexpr uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(MX_PAIR_N >> 3) << 17) | (1u << 23) | ((uint32_t)(MX_PAIR_M >> 4) << 24);
+    constexpr uint32_t idesc2 = idesc | (2u << 4) | (2u << 29);
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        ".reg .b32 t1, u0, u1;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "add.u64 a1, %1, 2;\n\t"
+        "add.u64 a2, %1, 4;\n\t"
+        "add.u64 a3, %1, 6;\n\t"
+        "add.u64 b1, %2, 2;\n\t"
+        "add.u64 b2, %2, 4;\n\t"
+        "add.u64 b3, %2, 6;\n\t"
+        "add.u32 t1, %3, 4;\n\t"
+        "add.u32 u0, %3, 8;\n\t"
+        "add.u32 u1, %3, 16;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %5, [%3], [u0], p;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a1, b1, %6, [%3], [u0], 1;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a2, b2, %5, [t1], [u1], 1;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a3, b3, %6, [t1], [u1], 1;\n\t"
+        "}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(sa), "r"(accumulate), "r"(idesc), "r"(idesc2)
+        : "memory");
+}
+
+template <typename TO>
 __global__ void __launch_bounds__(MX_THREADS, 1)
 gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                      const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_as,
                      TO *__restrict__ out, int n, int m, int chunks, int tiles_n, int tiles, int w_early)
 {
-    using Cfg = MxPairCfg<BN>;
-    constexpr int STAGES = Cfg::STAGES;
+    constexpr uint32_t STAGES = MX_PAIR_STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = (uint64_t *)(smem + STAGES * Cfg::STAGE_BYTES);
-    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 2);
+    const uint32_t codes0 = smem_u32(smem), scales0 = codes0 + STAGES * MX_PAIR_STAGE_BYTES;
+    uint64_t *bars = (uint64_t *)(smem + STAGES * MX_PAIR_STAGE_BYTES + MX_GROUPS * MX_PAIR_SCALE_BYTES);
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * STAGES, sc_full0 = empty0 + 8 * STAGES,
+                   sc_empty0 = sc_full0 + 8 * MX_GROUPS, accum = sc_empty0 + 8 * MX_GROUPS, drained = accum + 8;
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 2 * MX_GROUPS + 2);
     volatile int *abort = (volatile int *)(tmem_slot + 1);
 
     const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES),
-                   drained = smem_u32(bars + 2 * STAGES + 1);
     if (threadIdx.x == 0) {
         prefetch_tensor_map(&map_w);
         prefetch_tensor_map(&map_a);
         prefetch_tensor_map(&map_ws);
         prefetch_tensor_map(&map_as);
-        for (int s = 0; s < STAGES; s++) {
+        for (uint32_t s = 0; s < 2 * (STAGES + MX_GROUPS) + 1; s++)
             mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, 1);
-        }
-        mbar_init(accum, 1);
         mbar_init(drained, 16);             // the epilogue's warps of both CTAs
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -473,86 +513,86 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 
     if (warp == 0 && lane == 0) {
         // ---------------------------------------------------------- loads
-        uint32_t it = 0;
-        const uint32_t lead_full = cluster_addr(full0, 0);
-        bool ok = true, waited = false;
-        if (!w_early) {
+        uint32_t it = 0, group = 0;
+        const uint32_t lead_full = cluster_addr(full0, 0), lead_sc = cluster_addr(sc_full0, 0);
+        bool ok = true, waited = !w_early;
+        if (waited)
             pdl_wait();
-            waited = true;
-        }
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
-            const int m0 = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M, n0 = tile % tiles_n * BN;
-            const int ws = (m0 >> 7) * chunks, as = (n0 >> 7) * chunks;
+            const int m0 = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M, n0 = tile % tiles_n * MX_PAIR_N;
             for (int c = 0; c < chunks; c++, it++) {
-                const int s = it % STAGES;
+                const uint32_t s = it % STAGES, codes = codes0 + s * MX_PAIR_STAGE_BYTES;
+                const uint32_t g = group % MX_GROUPS, scales = scales0 + g * MX_PAIR_SCALE_BYTES;
+                const bool first = c % MX_GROUP == 0;
+                if (first) {
+                    if (group >= MX_GROUPS && !mbar_wait(sc_empty0 + 8 * g, ((group / MX_GROUPS) & 1) ^ 1, abort, &g_gemm_mx4_error, 7)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0)
+                        mbar_expect_tx(sc_full0 + 8 * g, 2 * MX_PAIR_SCALE_BYTES);
+                    tma_load_pair(scales, &map_ws, lead_sc + 8 * g, 0, 8 * c, m0 >> 7);
+                    group++;
+                }
                 if (it >= STAGES && !mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1, abort, &g_gemm_mx4_error, 1)) {
                     ok = false;
                     break;
                 }
-                const uint32_t dst = smem_u32(smem + s * Cfg::STAGE_BYTES), bar = lead_full + 8 * s;
                 if (rank == 0)
-                    mbar_expect_tx(full0 + 8 * s, 2 * Cfg::STAGE_BYTES);
-                tma_load_pair(dst, &map_w, bar, c * (MX4_CHUNK / 2), m0);
-                tma_load_pair(dst + MX_W_BYTES + Cfg::A_BYTES, &map_ws, bar, 0, ws + c);
+                    mbar_expect_tx(full0 + 8 * s, 2 * MX_PAIR_STAGE_BYTES);
+                tma_load_pair(codes, &map_w, lead_full + 8 * s, c * (MX4_CHUNK / 2), m0);
                 if (!waited) {
                     pdl_wait();
                     waited = true;
                 }
-                tma_load_pair(dst + MX_W_BYTES, &map_a, bar, c * (MX4_CHUNK / 2), n0 + (int)rank * (BN / 2));
-#pragma unroll
-                for (int t = 0; t < (BN + 127) / 128; t++)
-                    tma_load_pair(dst + MX_W_BYTES + Cfg::A_BYTES + MX4_TILE * (1 + t), &map_as, bar, 0, as + t * chunks + c);
+                if (first)
+                    tma_load_pair(scales + MX_GROUP * MX4_TILE, &map_as, lead_sc + 8 * g, 0, 8 * c, n0 >> 7);
+                tma_load_pair(codes + MX_W_BYTES, &map_a, lead_full + 8 * s, c * (MX4_CHUNK / 2), n0 + (int)rank * (MX_PAIR_N / 2));
             }
         }
         if (*abort && rank == 0) {
-            // the loads in flight of both CTAs: wait for each stage's last use, once, with the limit (the other CTA then
+            // the loads in flight of both CTAs: wait for each barrier's last use, once, with the limit (the other CTA then
             // waits for this one at the cluster's barrier)
             volatile int never = 0;
             for (uint32_t u = it > STAGES ? it - STAGES : 0; u < it; u++)
                 mbar_wait(full0 + 8 * (u % STAGES), (u / STAGES) & 1, &never, &g_gemm_mx4_error, 4);
+            for (uint32_t u = group > MX_GROUPS ? group - MX_GROUPS : 0; u < group; u++)
+                mbar_wait(sc_full0 + 8 * (u % MX_GROUPS), (u / MX_GROUPS) & 1, &never, &g_gemm_mx4_error, 4);
         }
     } else if (warp == 1 && rank == 0) {
         // --------------------------------------------------------------- MMAs of both CTAs
-        constexpr uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (1u << 23) | ((uint32_t)(MX_PAIR_M >> 4) << 24);
-        constexpr uint32_t idesc2 = idesc | (2u << 4) | (2u << 29);
-        const bool issue = elect_one();
-        uint32_t it = 0, done = 0;
+        uint32_t it = 0, group = 0, done = 0;
         bool ok = true;
         for (int tile = pair; tile < tiles && ok; tile += pairs, done++) {
-            if (done && !__all_sync(0xffffffffu, mbar_wait(drained, (done - 1) & 1, abort, &g_gemm_mx4_error, 6)))
-                break;
-            tc_fence_after();
             for (int c = 0; c < chunks; c++, it++) {
-                const int s = it % STAGES;
-                if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (it / STAGES) & 1, abort, &g_gemm_mx4_error, 2))) {
-                    ok = false;
+                const uint32_t s = it % STAGES, g = group % MX_GROUPS;
+                if (c % MX_GROUP == 0)
+                    ok = mbar_wait(sc_full0 + 8 * g, (group / MX_GROUPS) & 1, abort, &g_gemm_mx4_error, 8);
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(full0 + 8 * s, (it / STAGES) & 1, abort, &g_gemm_mx4_error, 2));
+                if (!ok)
                     break;
-                }
                 tc_fence_after();
-                const uint32_t base = smem_u32(smem) + s * Cfg::STAGE_BYTES, sc = base + MX_W_BYTES + Cfg::A_BYTES;
-                const uint32_t ca = tmem + BN + s * Cfg::SLOT_COLS, cb = ca + 8;
-                if (issue) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        mx_scales_pair(ca + 4 * h, sc + 512 * h);
-#pragma unroll
-                        for (int t = 0; t < (BN + 127) / 128; t++)      // a half's columns of all the rows side by side
-                            mx_scales_pair(cb + (BN + 127) / 128 * 4 * h + 4 * t, sc + MX4_TILE * (1 + t) + 512 * h);
-                    }
-                    const uint64_t da = smem_desc_sw128(base, 16, 1024), db = smem_desc_sw128(base + MX_W_BYTES, 16, 1024);
-#pragma unroll
-                    for (int h = 0; h < 4; h++)
-                        mx_mma_pair(tmem, da + 2 * h, db + 2 * h, h & 1 ? idesc2 : idesc, ca + 4 * (h >> 1),
-                                    cb + (BN + 127) / 128 * 4 * (h >> 1), c != 0 || h != 0);
+                const uint32_t codes = codes0 + s * MX_PAIR_STAGE_BYTES, col = tmem + MX_PAIR_N + s * MX_SLOT_COLS;
+                const uint32_t scales = scales0 + g * MX_PAIR_SCALE_BYTES + c % MX_GROUP * MX4_TILE;
+                mx_scales_pair(col, mx_scale_desc(scales), mx_scale_desc(scales + MX_GROUP * MX4_TILE));
+                if (c == 0 && done) {           // the accumulator of the tile before has been read
+                    ok = __all_sync(0xffffffffu, mbar_wait(drained, (done - 1) & 1, abort, &g_gemm_mx4_error, 6));
+                    if (!ok)
+                        break;
+                    tc_fence_after();
                 }
-                __syncwarp();
+                mx_chunk_pair(tmem, smem_desc_sw128(codes, 16, 1024), smem_desc_sw128(codes + MX_W_BYTES, 16, 1024), col, c != 0);
                 tc_commit_pair(empty0 + 8 * s);
+                if (c % MX_GROUP == MX_GROUP - 1 || c == chunks - 1) {
+                    tc_commit_pair(sc_empty0 + 8 * g);
+                    group++;
+                }
             }
             tc_commit_pair(accum);
         }
     } else if (warp >= 2) {
         // ------------------------------------------------------------ epilogue
-        constexpr int PART = BN / 2;
+        constexpr int PART = MX_PAIR_N / 2;
         const int q = warp & 3, part = (warp - 2) >> 2;
         const uint32_t lead_drained = cluster_addr(drained, 0);
         uint32_t done = 0;
@@ -561,7 +601,7 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             if (!__all_sync(0xffffffffu, mbar_wait(accum, done & 1, abort, &g_gemm_mx4_error, 3)))
                 break;
             tc_fence_after();
-            const int f = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M + q * 32 + lane, r0 = tile % tiles_n * BN + part * PART;
+            const int f = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M + q * 32 + lane, r0 = tile % tiles_n * MX_PAIR_N + part * PART;
             uint32_t v[PART];
 #pragma unroll
             for (int c = 0; c < PART; c += 32)
@@ -570,7 +610,7 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             tc_fence_before();
             __syncwarp();
             if (lane == 0)
-                mbar_arrive_cluster(lead_drained);
+                mbar_arrive_pair(lead_drained);
             if (f < m) {
                 TO *o = out + (size_t)r0 * m + f;
                 if (r0 + PART <= n) {
@@ -608,38 +648,39 @@ static bool mx_tensor_map(const void *codes, int rows, int k, int box_rows, CUte
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Scales as rows of 1,024 bytes, a chunk of 128 of the matrix's rows each.
-static bool mx_scale_map(const void *scales, int rows, int k, CUtensorMap *out)
+// Scales as [tiles of 128 rows, chunks, 1,024 bytes], in boxes of MX_GROUP chunks of box_tiles tiles; what lies outside
+// reads as zero.
+static bool mx_scale_map(const void *scales, int rows, int k, int box_tiles, CUtensorMap *out)
 {
     EncodeTiled enc = tensor_map_encoder();
     if (!enc)
         return false;
-    cuuint64_t dims[2] = {MX4_TILE / 4, (cuuint64_t)((rows + 127) / 128) * mx4_chunks(k)};
-    cuuint64_t strides[1] = {MX4_TILE};
-    cuuint32_t box[2] = {MX4_TILE / 4, 1}, estr[2] = {1, 1};
-    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(scales), dims, strides, box, estr,
+    const cuuint64_t chunks = mx4_chunks(k);
+    cuuint64_t dims[3] = {32, 8 * chunks, (cuuint64_t)((rows + 127) / 128)};
+    cuuint64_t strides[2] = {128, MX4_TILE * chunks};
+    cuuint32_t box[3] = {32, 8 * MX_GROUP, (cuuint32_t)box_tiles}, estr[3] = {1, 1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void *>(scales), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, typename TO>
+template <typename TO>
 static int launch_mx_pair(const void *ac, const void *as, const void *wc, const void *ws, TO *out, int n, int m, int k,
                           int w_early, cudaStream_t st)
 {
-    using Cfg = MxPairCfg<BN>;
     CUtensorMap map_w, map_a, map_ws, map_as;
-    if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || !mx_tensor_map(ac, n, k, BN / 2, &map_a) ||
-        !mx_scale_map(ws, m, k, &map_ws) || !mx_scale_map(as, n, k, &map_as))
+    if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || !mx_tensor_map(ac, n, k, MX_PAIR_N / 2, &map_a) ||
+        !mx_scale_map(ws, m, k, 1, &map_ws) || !mx_scale_map(as, n, k, MX_ROW_TILES, &map_as))
         return JB_EINVAL;
-    auto kern = gemm_mx4_pair_kernel<BN, TO>;
+    auto kern = gemm_mx4_pair_kernel<TO>;
     static unsigned long long allowed = 0;
-    if (!allow_dynamic_smem(kern, Cfg::SMEM_BYTES, allowed))
+    if (!allow_dynamic_smem(kern, MX_PAIR_SMEM, allowed))
         return JB_ELAUNCH;
-    const long long tiles_n = (n + BN - 1) / BN, tiles = tiles_n * ((m + MX_PAIR_M - 1) / MX_PAIR_M);
+    const long long tiles_n = (n + MX_PAIR_N - 1) / MX_PAIR_N, tiles = tiles_n * ((m + MX_PAIR_M - 1) / MX_PAIR_M);
     if (tiles > 0x7fffffff)
         return JB_EINVAL;
     const long long pairs = sm_count() / 2;
-    launch_cluster(kern, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), MX_THREADS, Cfg::SMEM_BYTES, st, 2u, map_w, map_a,
+    launch_cluster(kern, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), MX_THREADS, MX_PAIR_SMEM, st, 2u, map_w, map_a,
                    map_ws, map_as, out, n, m, mx4_chunks(k), (int)tiles_n, (int)tiles, w_early);
     return launch_status();
 }
@@ -693,9 +734,7 @@ static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, c
         return launch_mx<64, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 128)
         return launch_mx<128, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 256)
-        return launch_mx_pair<128, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
-    return launch_mx_pair<256, TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+    return launch_mx_pair<TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
 }
 
 static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, int out_dt, int n, int m, int k)
