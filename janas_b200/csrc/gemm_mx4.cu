@@ -347,8 +347,12 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 // tensor memory for scales; with 192 rows they would fit, but an MMA of 64 values of k takes 135 cycles whether it is of
 // 128, 192 or 256 rows: 2,048 rows x 18,944 x 2,560 52 us with tiles of 192.)
 //
-// What bounds it: the MMAs, with the loads close behind.  A copy of a chunk's scales costs a fifth of what a chunk's codes
-// do, however few its bytes, so one copy brings two chunks' scales.
+// What bounds it: the MMAs (541 cycles a chunk of 256 values of k, and 96 for the copies of its scales) and, while the
+// epilogue stores, what the SMs can take in from the L2 beside it.
+//
+// Tiles go round over the pairs; those that are left when less than a round is make up a last round in which each is
+// shared out along k by as many pairs as there are for it.  These write their sums to scratch, and a kernel behind this
+// one adds them up in the order of k.
 constexpr int MX_PAIR_M = 2 * MX_TILE_M;
 constexpr int MX_PAIR_N = 256;
 constexpr int MX_GROUP = 2;         // chunks whose scales are copied together
@@ -467,11 +471,35 @@ __device__ __forceinline__ void mx_chunk_pair(uint32_t d, uint64_t a, uint64_t b
         : "memory");
 }
 
+// What a pair does in its round `i`: a tile, a range of its chunks, and where its sums go.
+struct MxTask {
+    int tile, c0, c1, part;         // part: which of the partial sums in scratch, or -1: the output itself
+};
+
+// tiles: all tiles; whole: those that go round whole; splits: the pairs that share one of the others.
+struct MxSchedule {
+    int tiles_n, tiles, whole, splits;
+    __device__ __forceinline__ bool task(int i, int pair, int pairs, int chunks, MxTask &t) const
+    {
+        const long long u = (long long)i * pairs + pair;
+        if (u < whole) {
+            t = MxTask{(int)u, 0, chunks, -1};
+            return true;
+        }
+        // (whole is a multiple of the pairs wherever tiles are shared)
+        const int v = (int)(u - whole), left = v / splits, part = v - left * splits;
+        if (i > whole / pairs || left >= tiles - whole)
+            return false;
+        t = MxTask{whole + left, (int)((long long)chunks * part / splits), (int)((long long)chunks * (part + 1) / splits), v};
+        return true;
+    }
+};
+
 template <typename TO>
 __global__ void __launch_bounds__(MX_THREADS, 1)
 gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                      const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_as,
-                     TO *__restrict__ out, int n, int m, int chunks, int tiles_n, int tiles, int w_early)
+                     TO *__restrict__ out, float *__restrict__ partial, int n, int m, int chunks, const MxSchedule plan, int w_early)
 {
     constexpr uint32_t STAGES = MX_PAIR_STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -518,12 +546,13 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         bool ok = true, waited = !w_early;
         if (waited)
             pdl_wait();
-        for (int tile = pair; tile < tiles && ok; tile += pairs) {
-            const int m0 = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M, n0 = tile % tiles_n * MX_PAIR_N;
-            for (int c = 0; c < chunks; c++, it++) {
+        MxTask t;
+        for (int i = 0; ok && plan.task(i, pair, pairs, chunks, t); i++) {
+            const int m0 = t.tile / plan.tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M, n0 = t.tile % plan.tiles_n * MX_PAIR_N;
+            for (int c = t.c0; c < t.c1; c++, it++) {
                 const uint32_t s = it % STAGES, codes = codes0 + s * MX_PAIR_STAGE_BYTES;
                 const uint32_t g = group % MX_GROUPS, scales = scales0 + g * MX_PAIR_SCALE_BYTES;
-                const bool first = c % MX_GROUP == 0;
+                const bool first = (c - t.c0) % MX_GROUP == 0;
                 if (first) {
                     if (group >= MX_GROUPS && !mbar_wait(sc_empty0 + 8 * g, ((group / MX_GROUPS) & 1) ^ 1, abort, &g_gemm_mx4_error, 7)) {
                         ok = false;
@@ -563,8 +592,9 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         // --------------------------------------------------------------- MMAs of both CTAs
         uint32_t it = 0, group = 0, done = 0;
         bool ok = true;
-        for (int tile = pair; tile < tiles && ok; tile += pairs, done++) {
-            for (int c = 0; c < chunks; c++, it++) {
+        MxTask t;
+        for (; ok && plan.task(done, pair, pairs, chunks, t); done++) {
+            for (int c = 0; c < t.c1 - t.c0; c++, it++) {
                 const uint32_t s = it % STAGES, g = group % MX_GROUPS;
                 if (c % MX_GROUP == 0)
                     ok = mbar_wait(sc_full0 + 8 * g, (group / MX_GROUPS) & 1, abort, &g_gemm_mx4_error, 8);
@@ -583,7 +613,7 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 }
                 mx_chunk_pair(tmem, smem_desc_sw128(codes, 16, 1024), smem_desc_sw128(codes + MX_W_BYTES, 16, 1024), col, c != 0);
                 tc_commit_pair(empty0 + 8 * s);
-                if (c % MX_GROUP == MX_GROUP - 1 || c == chunks - 1) {
+                if (c % MX_GROUP == MX_GROUP - 1 || c == t.c1 - t.c0 - 1) {
                     tc_commit_pair(sc_empty0 + 8 * g);
                     group++;
                 }
@@ -597,11 +627,13 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         const uint32_t lead_drained = cluster_addr(drained, 0);
         uint32_t done = 0;
         pdl_wait();
-        for (int tile = pair; tile < tiles; tile += pairs, done++) {
+        MxTask t;
+        for (; plan.task(done, pair, pairs, chunks, t); done++) {
             if (!__all_sync(0xffffffffu, mbar_wait(accum, done & 1, abort, &g_gemm_mx4_error, 3)))
                 break;
             tc_fence_after();
-            const int f = tile / tiles_n * MX_PAIR_M + (int)rank * MX_TILE_M + q * 32 + lane, r0 = tile % tiles_n * MX_PAIR_N + part * PART;
+            const int fl = (int)rank * MX_TILE_M + q * 32 + lane;
+            const int f = t.tile / plan.tiles_n * MX_PAIR_M + fl, r0 = t.tile % plan.tiles_n * MX_PAIR_N + part * PART;
             uint32_t v[PART];
 #pragma unroll
             for (int c = 0; c < PART; c += 32)
@@ -611,7 +643,13 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             __syncwarp();
             if (lane == 0)
                 mbar_arrive_pair(lead_drained);
-            if (f < m) {
+            if (t.part >= 0) {
+                float *o = partial + ((size_t)t.part * MX_PAIR_N + part * PART) * MX_PAIR_M + fl;
+#pragma unroll
+                for (int j = 0; j < PART; j++)
+                    if (r0 + j < n)
+                        o[j * MX_PAIR_M] = __uint_as_float(v[j]);
+            } else if (f < m) {
                 TO *o = out + (size_t)r0 * m + f;
                 if (r0 + PART <= n) {
 #pragma unroll
@@ -632,6 +670,21 @@ gemm_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     cluster_wait();                 // neither CTA ends, or gives its tensor memory back, while the other's MMAs may run
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// The sums of tiles that were shared out along k: a block per row of a tile, a thread per feature.
+template <typename TO>
+__global__ void __launch_bounds__(MX_PAIR_M)
+mx_join_kernel(const float *partial, TO *__restrict__ out, int n, int m, const MxSchedule plan)
+{
+    pdl_trigger();
+    const int left = blockIdx.x / MX_PAIR_N, j = blockIdx.x - left * MX_PAIR_N, tile = plan.whole + left;
+    const int r = tile % plan.tiles_n * MX_PAIR_N + j, f = tile / plan.tiles_n * MX_PAIR_M + threadIdx.x;
+    if (r >= n || f >= m)
+        return;
+    pdl_wait();
+    const float *p = partial + ((size_t)left * plan.splits * MX_PAIR_N + j) * MX_PAIR_M + threadIdx.x;
+    out[(size_t)r * m + f] = from_f<TO>(add_partials(0.0f, p, plan.splits, (size_t)MX_PAIR_N * MX_PAIR_M));
 }
 
 // A matrix of codes in boxes of box_rows x 128 bytes with the 128-byte swizzle; what lies outside reads as zero.
@@ -664,9 +717,37 @@ static bool mx_scale_map(const void *scales, int rows, int k, int box_tiles, CUt
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How the tiles of a product are shared out.  What is left over after whole rounds is shared out along k where that saves
+// more than the partial sums' way through memory and a launch cost, about ten chunks' time (a chunk of k takes a pair 0.35
+// us; 2,048 rows x 2,560 x 9,728, 80 tiles of 38 chunks: 35 us in two rounds, 26 with six tiles shared by 12 pairs each).
+static MxSchedule mx_schedule(int n, int m, int k)
+{
+    const int pairs = sm_count() / 2, chunks = mx4_chunks(k);
+    MxSchedule p;
+    p.tiles_n = (n + MX_PAIR_N - 1) / MX_PAIR_N;
+    p.tiles = p.tiles_n * ((m + MX_PAIR_M - 1) / MX_PAIR_M);
+    p.whole = p.tiles;
+    p.splits = 1;
+    const int left = p.tiles % pairs;
+    if (left > 0) {
+        int splits = pairs / left;
+        splits = splits > chunks ? chunks : splits;
+        if (splits > 1 && chunks - (chunks + splits - 1) / splits > 10) {
+            p.whole = p.tiles - left;
+            p.splits = splits;
+        }
+    }
+    return p;
+}
+
+static long long mx_partial_bytes(const MxSchedule &p)
+{
+    return p.whole == p.tiles ? 0 : (long long)(p.tiles - p.whole) * p.splits * MX_PAIR_M * MX_PAIR_N * 4;
+}
+
 template <typename TO>
-static int launch_mx_pair(const void *ac, const void *as, const void *wc, const void *ws, TO *out, int n, int m, int k,
-                          int w_early, cudaStream_t st)
+static int launch_mx_pair(const void *ac, const void *as, const void *wc, const void *ws, TO *out, void *partial, int n, int m,
+                          int k, int w_early, cudaStream_t st)
 {
     CUtensorMap map_w, map_a, map_ws, map_as;
     if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || !mx_tensor_map(ac, n, k, MX_PAIR_N / 2, &map_a) ||
@@ -676,13 +757,18 @@ static int launch_mx_pair(const void *ac, const void *as, const void *wc, const 
     static unsigned long long allowed = 0;
     if (!allow_dynamic_smem(kern, MX_PAIR_SMEM, allowed))
         return JB_ELAUNCH;
-    const long long tiles_n = (n + MX_PAIR_N - 1) / MX_PAIR_N, tiles = tiles_n * ((m + MX_PAIR_M - 1) / MX_PAIR_M);
-    if (tiles > 0x7fffffff)
+    const MxSchedule plan = mx_schedule(n, m, k);
+    const int pairs = sm_count() / 2, shared = plan.tiles - plan.whole;
+    if (shared && !partial)
         return JB_EINVAL;
-    const long long pairs = sm_count() / 2;
-    launch_cluster(kern, dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs)), MX_THREADS, MX_PAIR_SMEM, st, 2u, map_w, map_a,
-                   map_ws, map_as, out, n, m, mx4_chunks(k), (int)tiles_n, (int)tiles, w_early);
-    return launch_status();
+    launch_cluster(kern, dim3(2u * (plan.tiles < pairs && !shared ? plan.tiles : pairs)), MX_THREADS, MX_PAIR_SMEM, st, 2u, map_w,
+                   map_a, map_ws, map_as, out, (float *)partial, n, m, mx4_chunks(k), plan, w_early);
+    int e = launch_status();
+    if (e == JB_OK && shared) {
+        launch(mx_join_kernel<TO>, (unsigned)shared * MX_PAIR_N, MX_PAIR_M, 0, st, (const float *)partial, out, n, m, plan);
+        e = launch_status();
+    }
+    return e;
 }
 
 // Parts of k (1, 2, 4 or 8) that a product's tiles are shared out in.
@@ -718,10 +804,11 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
 }
 
 constexpr int MX_ROWS_MOST = 32;    // rows that the product takes as floats
+constexpr int MX_FEW = 128;         // rows up to which a product's tiles are single CTAs'
 
 template <typename TO>
-static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, int n, int m, int k,
-                  int w_early, cudaStream_t st)
+static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, void *partial, int n,
+                  int m, int k, int w_early, cudaStream_t st)
 {
     if (rows.x)
         return n <= 16 ? launch_mx<16, TO, true>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
@@ -732,58 +819,78 @@ static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, c
         return launch_mx<32, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 64)
         return launch_mx<64, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 128)
+    if (n <= MX_FEW)
         return launch_mx<128, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    return launch_mx_pair<TO>(ac, as, wc, ws, out, n, m, k, w_early, st);
+    return launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
 }
 
-static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, int out_dt, int n, int m, int k)
+// Tiles and partial sums are counted in 32 bits.
+static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, const void *scratch, int out_dt, int n,
+                        int m, int k)
 {
-    return n < 0 || m < 0 || k < 1 || (out_dt != 0 && out_dt != 1) || (uintptr_t)ac % 16 || (uintptr_t)as % 16 ||
-           (uintptr_t)wc % 16 || (uintptr_t)ws % 16;
+    return n < 0 || m < 0 || k < 1 || (out_dt != 0 && out_dt != 1) || ((uintptr_t)ac | (uintptr_t)as | (uintptr_t)wc |
+           (uintptr_t)ws | (uintptr_t)scratch) % 16 || ((long long)n / 16 + 1) * ((long long)m / 128 + 1) > 0x3fffffff;
 }
 
 }  // namespace jb
 
 using namespace jb;
 
-// out [n, m] (out_dt 0 float32, 1 bfloat16) = a [n, k] . w [m, k]^T, both as codes and scales.  w_early: no kernel that
-// may still be running when this one starts writes the weights.
-extern "C" int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales, void *out,
-                             int out_dt, int n, int m, int k, int w_early, cudaStream_t st)
+// The most rows that jb_linear_mx4_rows packs in the product's own kernel.
+extern "C" int jb_linear_mx4_rows_most(void) { return MX_ROWS_MOST; }
+
+// Bytes of scratch that a product needs, with n rows that come as codes (rows 0) or as floats (rows 1).
+extern "C" long long jb_linear_mx4_scratch(int n, int m, int k, int rows)
 {
-    if (bad_product(a_codes, a_scales, w_codes, w_scales, out_dt, n, m, k))
+    if (n < 1 || m < 1 || k < 1)
+        return 0;
+    long long bytes = n > MX_FEW ? mx_partial_bytes(mx_schedule(n, m, k)) : 0;
+    if (rows && n > MX_ROWS_MOST)
+        bytes += jb_mx4_code_bytes(n, k) + jb_mx4_scale_bytes(n, k);
+    return bytes;
+}
+
+// How many kernels such a product launches.
+extern "C" int jb_linear_mx4_launches(int n, int m, int k, int rows)
+{
+    if (n < 1 || m < 1 || k < 1)
+        return 0;
+    return 1 + (rows && n > MX_ROWS_MOST) + (n > MX_FEW && mx_partial_bytes(mx_schedule(n, m, k)) > 0);
+}
+
+// out [n, m] (out_dt 0 float32, 1 bfloat16) = a [n, k] . w [m, k]^T, both as codes and scales.  scratch: see
+// jb_linear_mx4_scratch.  w_early: no kernel that may still be running when this one starts writes the weights.
+extern "C" int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales, void *out,
+                             int out_dt, int n, int m, int k, void *scratch, int w_early, cudaStream_t st)
+{
+    if (bad_product(a_codes, a_scales, w_codes, w_scales, scratch, out_dt, n, m, k))
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;
     const MxRows none{nullptr, k, 0, 0};
-    return out_dt == 1 ? any_mx(a_codes, a_scales, none, w_codes, w_scales, (bf16 *)out, n, m, k, w_early, st)
-                       : any_mx(a_codes, a_scales, none, w_codes, w_scales, (float *)out, n, m, k, w_early, st);
+    return out_dt == 1 ? any_mx(a_codes, a_scales, none, w_codes, w_scales, (bf16 *)out, scratch, n, m, k, w_early, st)
+                       : any_mx(a_codes, a_scales, none, w_codes, w_scales, (float *)out, scratch, n, m, k, w_early, st);
 }
 
-// The most rows that jb_linear_mx4_rows needs no scratch for.
-extern "C" int jb_linear_mx4_rows_most(void) { return MX_ROWS_MOST; }
-
 // The same with a as floats (dt 0 float32, 1 bfloat16), which are brought to 4 bits on the way: in the product's own
-// kernel for up to jb_linear_mx4_rows_most() rows, else by a kernel ahead of it, in scratch (jb_mx4_code_bytes and
-// jb_mx4_scale_bytes of [n, k], one behind the other).
-extern "C" int jb_linear_mx4_rows(const void *x, int dt, void *scratch, const void *w_codes, const void *w_scales, void *out,
-                                  int out_dt, int n, int m, int k, int w_early, cudaStream_t st)
+// kernel for up to jb_linear_mx4_rows_most() rows, else by a kernel ahead of it, in scratch.
+extern "C" int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, const void *w_scales, void *out, int out_dt, int n,
+                                  int m, int k, void *scratch, int w_early, cudaStream_t st)
 {
-    if (bad_product(scratch, nullptr, w_codes, w_scales, out_dt, n, m, k) || (dt != 0 && dt != 1))
+    if (bad_product(nullptr, nullptr, w_codes, w_scales, scratch, out_dt, n, m, k) || (dt != 0 && dt != 1))
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;
     if (n > MX_ROWS_MOST) {
         if (!scratch)
             return JB_EINVAL;
-        void *scales = (uint8_t *)scratch + jb_mx4_code_bytes(n, k);
-        const int e = jb_mx4_quantize(x, dt, scratch, scales, n, k, 1, st);
-        return e != JB_OK ? e : jb_linear_mx4(scratch, scales, w_codes, w_scales, out, out_dt, n, m, k, w_early, st);
+        uint8_t *codes = (uint8_t *)scratch, *scales = codes + jb_mx4_code_bytes(n, k), *rest = scales + jb_mx4_scale_bytes(n, k);
+        const int e = jb_mx4_quantize(x, dt, codes, scales, n, k, 1, st);
+        return e != JB_OK ? e : jb_linear_mx4(codes, scales, w_codes, w_scales, out, out_dt, n, m, k, rest, w_early, st);
     }
     const MxRows rows{x, k, dt, k % 8 == 0 && (uintptr_t)x % 16 == 0};
-    return out_dt == 1 ? any_mx(nullptr, nullptr, rows, w_codes, w_scales, (bf16 *)out, n, m, k, w_early, st)
-                       : any_mx(nullptr, nullptr, rows, w_codes, w_scales, (float *)out, n, m, k, w_early, st);
+    return out_dt == 1 ? any_mx(nullptr, nullptr, rows, w_codes, w_scales, (bf16 *)out, nullptr, n, m, k, w_early, st)
+                       : any_mx(nullptr, nullptr, rows, w_codes, w_scales, (float *)out, nullptr, n, m, k, w_early, st);
 }
 
 // Reads and clears the error word: 0, or which wait ran out first (as jb_gemm_tc_error).

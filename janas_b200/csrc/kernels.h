@@ -171,10 +171,12 @@ int jb_mx4_gated_unit(const float *z, int S, long long stride, void *codes, void
                       float alpha, float limit, float shift, cudaStream_t st);
 int jb_mx4_values(const void *codes, const void *scales, void *out, int out_dt, int n, int k, cudaStream_t st);
 int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales, void *out,
-                  int out_dt, int n, int m, int k, int w_early, cudaStream_t st);
+                  int out_dt, int n, int m, int k, void *scratch, int w_early, cudaStream_t st);
+int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, const void *w_scales, void *out, int out_dt,
+                       int n, int m, int k, void *scratch, int w_early, cudaStream_t st);
 int jb_linear_mx4_rows_most(void);
-int jb_linear_mx4_rows(const void *x, int dt, void *scratch, const void *w_codes, const void *w_scales, void *out,
-                       int out_dt, int n, int m, int k, int w_early, cudaStream_t st);
+long long jb_linear_mx4_scratch(int n, int m, int k, int rows);
+int jb_linear_mx4_launches(int n, int m, int k, int rows);
 int jb_gemm_mx4_error(void);
 int jb_short_conv(const float *x, const float *w, float *state, long long slot_stride, const int32_t *row_pos,
                   const int32_t *row_seq, const int32_t *seq_slot, void *out, int out_dt, int n,

@@ -1443,6 +1443,9 @@ def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
+_MX4_ROWS = 32      # up to as many rows a 4-bit product needs no scratch (jb_linear_mx4_rows_most)
+
+
 def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """a [n, k] . w [m, k]^T with both in microscaled 4-bit floats, summed in float32: [n, m] in float32 or
     bfloat16, the result itself and no stack of parts.  ``a``: an Mx4, or float32 or bfloat16 rows, which are
@@ -1454,26 +1457,31 @@ def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tenso
     m, k = w.rows, w.k
     st = _stream_of(w._buf, "weight")
     L = lib()
-    if a.__class__ is Mx4:
+    packed = a.__class__ is Mx4
+    if packed:
         if a.k != k:
             raise KernelError(f"linear_mx4: rows of {a.k} values and a weight of {k}")
-        if a._buf.get_device() != w._buf.get_device():
-            raise KernelError("linear_mx4: the rows and the weight are on different devices")
-        n = a.rows
-        out = w._buf.new_empty((n, m), dtype=out_dtype)
-        _check(L.jb_linear_mx4(a._at_codes, a._at_scales, w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k,
-                               w.settled, st), "linear_mx4", 1 if n and m else 0)
-        return out
-    _need(a, "activations", _FLOATS, (None, k))
-    if a.get_device() != w._buf.get_device():
+        n, at = a.rows, a._buf
+    else:
+        _need(a, "activations", _FLOATS, (None, k))
+        n, at = a.shape[0], a
+    if at.get_device() != w._buf.get_device():
         raise KernelError("linear_mx4: the rows and the weight are on different devices")
-    n = a.shape[0]
-    out = a.new_empty((n, m), dtype=out_dtype)
-    few = n <= L.jb_linear_mx4_rows_most()
-    scratch = None if few or not m else Mx4._new(n, k, a, False)
-    _check(L.jb_linear_mx4_rows(a.data_ptr(), _DT[a.dtype], None if scratch is None else scratch._at_codes, w._at_codes,
-                                w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k, w.settled, st), "linear_mx4",
-           (1 if few else 2) if n and m else 0)
+    out = at.new_empty((n, m), dtype=out_dtype)
+    scratch, launches = None, 1
+    if n > _MX4_ROWS:
+        have = L.jb_linear_mx4_scratch(n, m, k, not packed)
+        if have:
+            scratch = at.new_empty(have, dtype=torch.uint8)
+            launches = L.jb_linear_mx4_launches(n, m, k, not packed)
+    at_scratch = None if scratch is None else scratch.data_ptr()
+    if packed:
+        code = L.jb_linear_mx4(a._at_codes, a._at_scales, w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k,
+                               at_scratch, w.settled, st)
+    else:
+        code = L.jb_linear_mx4_rows(a.data_ptr(), _DT[a.dtype], w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m,
+                                    k, at_scratch, w.settled, st)
+    _check(code, "linear_mx4", launches if n and m else 0)
     return out
 
 

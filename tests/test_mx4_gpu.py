@@ -409,3 +409,20 @@ def test_no_rows():
     one = torch.ones(96, device=DEV)
     assert o.norm_residual_norm(e, e.clone(), one, one, 1e-5, out="mx4").shape == (0, 96)
     assert o.mx4_gated_unit(torch.empty((0, 96), device=DEV)).shape == (0, 48)
+
+
+# the last: 237 tiles on 74 pairs leave 15, four pairs for each; sharing 12 chunks of k among four saves nine, too few
+@pytest.mark.parametrize("n,m,k,launches", [(300, 700, 9728, 2), (2048, 2560, 4096, 2), (140, 257, 40000, 2),
+                                            (600, 20000, 3000, 1)])
+def test_linear_shared_tiles(n, m, k, launches):
+    """Products whose last tiles are shared out along k: the same sums, once more the same bits, and rows that do not
+    depend on how many there are beyond the rounding of the parts' sums."""
+    o, a, w, av, wv = product_case(n, m, k)
+    assert o.lib().jb_linear_mx4_launches(n, m, k, 0) == launches
+    qa, qw = o.mx4_quantize(a.to(DEV)), o.mx4_quantize(w.to(DEV))
+    got = o.linear_mx4(qa, qw)
+    some = torch.randperm(n, generator=torch.Generator().manual_seed(1))[:40]
+    want, tol = av[some] @ wv.T, product_bound(av[some], wv, k)
+    assert ((got.cpu().double()[some] - want).abs() <= tol).all()
+    assert torch.equal(got, o.linear_mx4(qa, qw)) and torch.equal(got.to(BF16), o.linear_mx4(qa, qw, BF16))
+    assert o.gemm_tc_error() == 0
