@@ -1,7 +1,8 @@
 // Rows and matrices brought to microscaled 4-bit floats (mx4.cuh), and back.
 //
-// A warp takes a chunk of 256 values of a row, eight to a lane: four lanes make a block, whose largest magnitude they
-// find by two shuffles; the lane's codes are one word.  Bound by memory: a value read, 17 / 32 of a byte written.
+// Rows that whole 16-byte loads fit: a warp takes 512 values of a row, sixteen to a lane, so two lanes make a block and one
+// shuffle finds its largest magnitude.  Others, and the gated unit: 256 values, eight to a lane.  Bound by the instructions
+// it takes to scale, round and pack (and for the unit by its exponential and division), close to what memory takes.
 //
 // The kernel that quantizes a caller's rows may be followed by a product that reads them as its weights ahead of its
 // dependency wait, so unless `early` is set it lets no kernel behind it start before it has ended, and its stores stand
@@ -11,7 +12,7 @@
 
 namespace jb {
 
-template <typename T, bool VEC> struct RowSource {
+template <typename T> struct RowSource {
     const T *x;
     int k;
     struct Values {
@@ -19,20 +20,9 @@ template <typename T, bool VEC> struct RowSource {
     };
     __device__ __forceinline__ void load(size_t r, int col0, Values &t) const
     {
-        load8<T, VEC>(x + r * (size_t)k + col0, k - col0, t.v);
+        load8<T, false>(x + r * (size_t)k + col0, k - col0, t.v);
     }
     __device__ __forceinline__ uint32_t pack(Values &t, uint32_t &code) const { return mx4_pack_chunk(t.v, code); }
-};
-
-template <> struct RowSource<bf16, true> {
-    const bf16 *x;
-    int k;
-    typedef uint4 Values;
-    __device__ __forceinline__ void load(size_t r, int col0, Values &t) const
-    {
-        t = col0 < k ? *reinterpret_cast<const uint4 *>(x + r * (size_t)k + col0) : make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ uint32_t pack(Values &t, uint32_t &code) const { return mx4_pack_chunk(t, code); }
 };
 
 // The gated unit of the sums [S, n, 2 k]: columns [0, k) the gate, [k, 2 k) the up side.
@@ -69,39 +59,92 @@ template <bool VEC> struct UnitSource {
     }
 };
 
-// A warp takes U chunks that follow one another at a time, all read before the first is packed.  `total`: n times the
-// chunks of a row.
-template <typename Source, int U>
+// Sixteen values of a lane as they are packed: floats, or bfloat16 as they lie in memory; zeros past the row's end.
+struct Sixteen {
+    float v[16];
+    __device__ __forceinline__ void load(const float *p, int left)
+    {
+        load8<float, true>(p, left, v);
+        load8<float, true>(p + 8, left - 8, v + 8);
+    }
+    __device__ __forceinline__ uint2 pack(uint32_t &code) const { return mx4_pack16(v, code); }
+};
+struct SixteenBf16 {
+    uint4 v[2];
+    __device__ __forceinline__ void load(const bf16 *p, int left)
+    {
+        const uint4 *q = reinterpret_cast<const uint4 *>(p);
+        v[0] = left > 0 ? q[0] : make_uint4(0, 0, 0, 0);
+        v[1] = left > 8 ? q[1] : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ uint2 pack(uint32_t &code) const { return mx4_pack16(v, code); }
+};
+
+// total: n times the spans of 512 values of a row.  A warp takes U spans at a time, all read before the first is packed.
+template <typename T, typename Values, int U>
 __global__ void __launch_bounds__(256)
-mx4_quantize_kernel(const Source src, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, unsigned total, int k, int early)
+mx4_rows_kernel(const T *x, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, unsigned total, int k, int early)
 {
     if (early)
         pdl_trigger();
     pdl_wait();
-    const unsigned chunks = mx4_chunks(k), step = gridDim.x * (blockDim.x >> 5) * U;
+    constexpr int SPAN = 2 * MX4_CHUNK;
+    const int lane = threadIdx.x & 31, chunks = mx4_chunks(k);
+    const unsigned spans = (unsigned)(chunks + 1) / 2, step = gridDim.x * (blockDim.x >> 5) * U;
+    const size_t row_bytes = mx4_row_bytes(k);
     for (unsigned first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * U; first < total;) {
-        typename Source::Values v[U];
-        unsigned r = first / chunks, c = first - r * chunks, r0 = r, q0 = c;
+        Values v[U];
+        unsigned r = first / spans, c = first - r * spans, r0 = r, q0 = c;
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            const int col0 = (int)c * SPAN + 16 * lane;
             if (first + u < total)
-                src.load(r, c * MX4_CHUNK + 8 * (threadIdx.x & 31), v[u]);
-            if (++c == chunks)
+                v[u].load(x + r * (size_t)k + col0, k - col0);
+            if (++c == spans)
                 c = 0, r++;
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (first + u < total) {
                 uint32_t code;
-                const uint32_t packed = src.pack(v[u], code);
-                mx4_store_chunk(packed, code, r0, q0, k, codes, scales);
+                const uint2 packed = v[u].pack(code);
+                const unsigned at = q0 * (SPAN / 2) + 8 * lane;
+                if (at < row_bytes)
+                    *reinterpret_cast<uint2 *>(codes + r0 * row_bytes + at) = packed;
+                const int ch = 2 * (int)q0 + (lane >> 4);
+                if ((lane & 1) == 0 && ch < chunks)
+                    scales[mx4_scale_at(r0, ch, chunks, (lane >> 3) & 1) + ((lane >> 1) & 3)] = (uint8_t)code;
             }
-            if (++q0 == chunks)
+            if (++q0 == spans)
                 q0 = 0, r0++;
         }
         if (total - first <= step)
             break;
         first += step;
+    }
+    if (!early)
+        __threadfence();
+}
+
+// A warp takes a chunk at a time.  total: n times the chunks of a row.
+template <typename Source>
+__global__ void __launch_bounds__(256)
+mx4_quantize_kernel(const Source src, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, unsigned total, int k, int early)
+{
+    if (early)
+        pdl_trigger();
+    pdl_wait();
+    const unsigned chunks = mx4_chunks(k), step = gridDim.x * (blockDim.x >> 5);
+    for (unsigned i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total;) {
+        typename Source::Values v;
+        const unsigned r = i / chunks, c = i - r * chunks;
+        uint32_t code;
+        src.load(r, c * MX4_CHUNK + 8 * (threadIdx.x & 31), v);
+        const uint32_t packed = src.pack(v, code);
+        mx4_store_chunk(packed, code, r, c, k, codes, scales);
+        if (total - i <= step)
+            break;
+        i += step;
     }
     if (!early)
         __threadfence();
@@ -152,15 +195,27 @@ mx4_values_kernel(const uint8_t *codes, const uint8_t *scales, T *__restrict__ o
 static int mx4_unroll(size_t total) { return total >= (size_t)sm_count() * 32 * 4 ? 4 : 1; }
 static unsigned mx4_grid(size_t total, int unroll) { return (unsigned)((total + 8 * unroll - 1) / (8 * unroll)); }
 
-template <typename Source, int U>
+template <typename Source>
 static int quantize(const Source &src, void *codes, void *scales, int n, int k, int early, cudaStream_t st)
 {
     const size_t total = (size_t)n * mx4_chunks(k);
     if (total > 0xffffff00u)
         return JB_EINVAL;
-    const int u = mx4_unroll(total) > 1 ? U : 1;
+    const unsigned most = (unsigned)sm_count() * 8, grid = mx4_grid(total, 1);
+    launch(mx4_quantize_kernel<Source>, grid < most ? grid : most, 256, 0, st, src, (uint8_t *)codes, (uint8_t *)scales,
+           (unsigned)total, k, early);
+    return launch_status();
+}
+
+template <typename T, typename Values>
+static int quantize_rows(const T *x, void *codes, void *scales, int n, int k, int early, cudaStream_t st)
+{
+    const size_t total = (size_t)n * ((mx4_chunks(k) + 1) / 2);
+    if (total > 0xffffff00u)
+        return JB_EINVAL;
+    const int u = mx4_unroll(total) > 1 ? 2 : 1;
     const unsigned most = (unsigned)sm_count() * 8, grid = mx4_grid(total, u);
-    launch(u > 1 ? mx4_quantize_kernel<Source, U> : mx4_quantize_kernel<Source, 1>, grid < most ? grid : most, 256, 0, st, src,
+    launch(u > 1 ? mx4_rows_kernel<T, Values, 2> : mx4_rows_kernel<T, Values, 1>, grid < most ? grid : most, 256, 0, st, x,
            (uint8_t *)codes, (uint8_t *)scales, (unsigned)total, k, early);
     return launch_status();
 }
@@ -201,11 +256,11 @@ extern "C" int jb_mx4_quantize(const void *x, int dt, void *codes, void *scales,
     if (n == 0)
         return JB_OK;
     const bool vec = k % 8 == 0 && (uintptr_t)x % 16 == 0;
-#define JB_Q(T, V) quantize<RowSource<T, V>, 4>(RowSource<T, V>{(const T *)x, k}, codes, scales, n, k, early, st)
     if (dt == 1)
-        return vec ? JB_Q(bf16, true) : JB_Q(bf16, false);
-    return vec ? JB_Q(float, true) : JB_Q(float, false);
-#undef JB_Q
+        return vec ? quantize_rows<bf16, SixteenBf16>((const bf16 *)x, codes, scales, n, k, early, st)
+                   : quantize(RowSource<bf16>{(const bf16 *)x, k}, codes, scales, n, k, early, st);
+    return vec ? quantize_rows<float, Sixteen>((const float *)x, codes, scales, n, k, early, st)
+               : quantize(RowSource<float>{(const float *)x, k}, codes, scales, n, k, early, st);
 }
 
 // The gated unit (see jb_gated_unit) of z, a stack [S, n, 2 ff] of sums, in 4 bits.
@@ -218,8 +273,8 @@ extern "C" int jb_mx4_gated_unit(const float *z, int S, long long stride, void *
         return JB_OK;
     const GatedUnit unit{alpha, limit, shift};
     if (ff % 8 == 0 && (uintptr_t)z % 16 == 0 && stride % 4 == 0)
-        return quantize<UnitSource<true>, 2>(UnitSource<true>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
-    return quantize<UnitSource<false>, 2>(UnitSource<false>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
+        return quantize(UnitSource<true>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
+    return quantize(UnitSource<false>{z, S, (size_t)stride, ff, unit}, codes, scales, n, ff, 1, st);
 }
 
 // What codes and scales stand for, as [n, k].

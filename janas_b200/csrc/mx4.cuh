@@ -81,14 +81,18 @@ __device__ __forceinline__ float mx4_larger(float a, float b)
     return m;
 }
 
+__device__ __forceinline__ float mx4_largest(float a, float b, float c)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
 // The bits of the largest magnitude among eight values.
 __device__ __forceinline__ uint32_t mx4_top8(const float *v)
 {
-    float t = fabsf(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; i++)
-        t = mx4_larger(t, fabsf(v[i]));
-    return __float_as_uint(t);
+    const float a = mx4_largest(fabsf(v[0]), fabsf(v[1]), fabsf(v[2])), b = mx4_largest(fabsf(v[3]), fabsf(v[4]), fabsf(v[5]));
+    return __float_as_uint(mx4_larger(mx4_largest(a, b, fabsf(v[6])), fabsf(v[7])));
 }
 
 // Eight consecutive floats of which `left` exist; zeros for the others.  VEC: all eight or none, at a 16-byte boundary.
@@ -128,15 +132,19 @@ __device__ __forceinline__ uint32_t mx4_pack_chunk(const float *v, uint32_t &cod
     return mx4_pack8(v, mx4_inverse(code));
 }
 
-// The same for eight bfloat16 as they lie in memory: magnitudes and the products with a power of two two at a time.
-__device__ __forceinline__ uint32_t mx4_pack_chunk(const uint4 &x, uint32_t &code)
+// Sixteen values of a lane, half a block: two words of codes, and the block's scale's code, which two lanes share.
+__device__ __forceinline__ uint2 mx4_pack16(const float *v, uint32_t &code)
 {
-    uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    top = max(top & 0xffff0000u, top << 16);
+    uint32_t top = max(mx4_top8(v), mx4_top8(v + 8));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     code = mx4_scale_code(top);
-    const uint32_t inv = (254u - min(code, 252u)) * 0x00800080u;
+    const float inv = mx4_inverse(code);
+    return make_uint2(mx4_pack8(v, inv), mx4_pack8(v + 8, inv));
+}
+
+// Eight bfloat16 times a power of two (in both halves of inv), in 4 bits.
+__device__ __forceinline__ uint32_t mx4_pack8(const uint4 &x, uint32_t inv)
+{
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     float v[8];
 #pragma unroll
@@ -147,6 +155,21 @@ __device__ __forceinline__ uint32_t mx4_pack_chunk(const uint4 &x, uint32_t &cod
         v[2 * i + 1] = __uint_as_float(p & 0xffff0000u);
     }
     return mx4_pack8(v);
+}
+
+// The same for sixteen bfloat16 as they lie in memory: magnitudes and the products with a power of two two at a time.
+__device__ __forceinline__ uint2 mx4_pack16(const uint4 *x, uint32_t &code)
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
+                                     __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top & 0xffff0000u, top << 16);
+    code = mx4_scale_code(top);
+    const uint32_t inv = (254u - min(code, 252u)) * 0x00800080u;
+    return make_uint2(mx4_pack8(x[0], inv), mx4_pack8(x[1], inv));
 }
 
 // A lane's four values of a block that eight lanes share, in 16 bits, and the block's scale's code.
