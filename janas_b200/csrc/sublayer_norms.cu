@@ -12,8 +12,11 @@
 // N: a layer norm (t - mean) / sqrt(var + eps) * w + b, var the mean of the squared deviations, or with `rms`
 // t / sqrt(mean(t^2) + eps) * w + b.  h is float32, bfloat16 or microscaled 4-bit floats (mx4.cuh).
 //
-// Bound by memory, and by the chain of sums for few rows.  A block per row, which stays in registers between the sums, up to
-// four groups of four values a thread; rows that whole 16-byte loads do not fit, or longer ones, stay in shared memory.
+// Bound by instructions and memory, and for few rows by the chain of sums.  A block per row, which stays in registers between
+// the sums, two groups of four values a thread (2,048 rows of 2,560 with a gate, from memory: 31 us; with five groups and a
+// quarter of the warps 42, with one group 37, though 8 rows then take 3.5 instead of 4.7; with each block's next row
+// prefetched into shared memory 36).  Rows that whole
+// 16-byte loads do not fit, or longer ones, stay in shared memory.
 // How a row is shared out among the threads depends on its length alone, so its bits are the same in any batch.
 #include "kernels.h"
 #include "mx4.cuh"
@@ -32,7 +35,7 @@ struct NormsArgs {
     uint8_t *scales;
 };
 
-__device__ __forceinline__ float gated(float v, float z) { return __fmul_rn(v, 1.0f / (1.0f + expf(-z))); }
+__device__ __forceinline__ float gated(float v, float z) { return __fmul_rn(v, __frcp_rn(1.0f + expf(-z))); }
 // t inv w (+ b), and x + c t
 __device__ __forceinline__ float normed(float t, float inv, float w, const float *b)
 {
@@ -54,22 +57,29 @@ __device__ __forceinline__ void row_moments(const float *row, int dm, float sum,
     inv = rsqrtf(block_sum(sq, red) * (1.0f / dm) + eps);
 }
 
-// The block's sum of v: every warp adds up all warps' sums from a slot that no other sum uses, so one barrier is enough.
-__device__ __forceinline__ float slot_sum(float v, float *slot)
+// The sum of v over a block of at most W warps: every thread adds up all warps' sums, in order, from slots that no other sum
+// uses (zeros where there is no warp), so one barrier is enough.
+template <int W>
+__device__ __forceinline__ float slot_sum(float v, float *slots)
 {
-    const int lane = threadIdx.x & 31;
     v = warp_sum(v);
-    if (lane == 0)
-        slot[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0)
+        slots[threadIdx.x >> 5] = v;
     __syncthreads();
-    return warp_sum(lane < (int)(blockDim.x >> 5) ? slot[lane] : 0.0f);
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w += 4) {
+        const float4 u = load4(slots + w);
+        t += (u.x + u.y) + (u.z + u.w);
+    }
+    return t;
 }
 
 __device__ __forceinline__ float sum4(const float4 &v) { return (v.x + v.y) + (v.z + v.w); }
 
 // The norm of a row in registers: t <- (t - mean) / sqrt(var + eps) * w + b.  Values past the row's end are zeros before
 // and whatever comes out after.
-template <int NV>
+template <int NV, int W>
 __device__ __forceinline__ void norm_row(float4 *t, int dm, bool rms, float eps, const float *w, const float *b, float *slots)
 {
     float mean = 0.0f;
@@ -78,7 +88,7 @@ __device__ __forceinline__ void norm_row(float4 *t, int dm, bool rms, float eps,
 #pragma unroll
         for (int j = 0; j < NV; j++)
             sum += sum4(t[j]);
-        mean = slot_sum(sum, slots) * (1.0f / dm);
+        mean = slot_sum<W>(sum, slots) * (1.0f / dm);
     }
     float sq = 0.0f;
 #pragma unroll
@@ -88,7 +98,7 @@ __device__ __forceinline__ void norm_row(float4 *t, int dm, bool rms, float eps,
             sq += (t[j].x * t[j].x + t[j].y * t[j].y) + (t[j].z * t[j].z + t[j].w * t[j].w);
         }
     }
-    const float inv = rsqrtf(slot_sum(sq, slots + 32) * (1.0f / dm) + eps);
+    const float inv = rsqrtf(slot_sum<W>(sq, slots + W) * (1.0f / dm) + eps);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = 4 * (threadIdx.x + j * blockDim.x);
@@ -119,33 +129,14 @@ __device__ __forceinline__ float4 sum_stack(const float *bias, const float *p, i
     return v;
 }
 
-// NV groups of four values a thread; every address at a 16-byte boundary.
-template <int NV>
-__global__ void __launch_bounds__(1024)
-sublayer_norms_vec_kernel(const NormsArgs a)
+// From the gated sums t and the old x of a row: x and h.
+template <int NV, int W>
+__device__ __forceinline__ void finish_row(const NormsArgs &a, size_t r, float4 *t, const float4 *old, float (*slots)[W])
 {
-    __shared__ float slots[4][32];
-    pdl_trigger();
-    pdl_wait();
-    const size_t r = blockIdx.x;
     const int dm = a.dm;
     float *x = a.x + r * dm;
-    float4 t[NV], old[NV];
-#pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int i = 4 * (threadIdx.x + j * blockDim.x);
-        t[j] = old[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < dm) {
-            old[j] = load4(x + i);
-            t[j] = sum_stack(a.y_bias ? a.y_bias + i : nullptr, a.y + r * dm + i, a.Sy, a.y_stride);
-            if (a.g) {
-                const float4 z = sum_stack(a.g_bias ? a.g_bias + i : nullptr, a.g + r * a.g_ld + a.g_col0 + i, a.Sg, a.g_stride);
-                t[j] = make_float4(gated(t[j].x, z.x), gated(t[j].y, z.y), gated(t[j].z, z.z), gated(t[j].w, z.w));
-            }
-        }
-    }
     if (a.w1)
-        norm_row<NV>(t, dm, a.rms, a.eps1, a.w1, a.b1, slots[0]);
+        norm_row<NV, W>(t, dm, a.rms, a.eps1, a.w1, a.b1, slots[0]);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = 4 * (threadIdx.x + j * blockDim.x);
@@ -158,7 +149,7 @@ sublayer_norms_vec_kernel(const NormsArgs a)
     }
     if (!a.w2)
         return;
-    norm_row<NV>(t, dm, a.rms, a.eps2, a.w2, a.b2, slots[2]);
+    norm_row<NV, W>(t, dm, a.rms, a.eps2, a.w2, a.b2, slots[2]);
     const int blocks = (dm + 31) / 32, chunks = mx4_chunks(dm);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -184,6 +175,38 @@ sublayer_norms_vec_kernel(const NormsArgs a)
         if (b < 8 * chunks)
             a.scales[mx4_scale_at(r, b >> 3, chunks, (b >> 2) & 1) + (b & 3)] = 0;
     }
+}
+
+__device__ __forceinline__ float4 gated4(const float4 &v, const float4 &z)
+{
+    return make_float4(gated(v.x, z.x), gated(v.y, z.y), gated(v.z, z.z), gated(v.w, z.w));
+}
+
+// NV groups of four values a thread, at most W warps; every address at a 16-byte boundary.
+template <int NV, int W>
+__global__ void __launch_bounds__(32 * W)
+sublayer_norms_vec_kernel(const NormsArgs a)
+{
+    __shared__ __align__(16) float slots[4][W];
+    if (threadIdx.x < 4 * W)
+        slots[0][threadIdx.x] = 0.0f;
+    pdl_trigger();
+    __syncthreads();
+    pdl_wait();
+    const size_t r = blockIdx.x;
+    float4 t[NV], old[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = 4 * (threadIdx.x + j * blockDim.x);
+        t[j] = old[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < a.dm) {
+            old[j] = load4(a.x + r * a.dm + i);
+            t[j] = sum_stack(a.y_bias ? a.y_bias + i : nullptr, a.y + r * a.dm + i, a.Sy, a.y_stride);
+            if (a.g)
+                t[j] = gated4(t[j], sum_stack(a.g_bias ? a.g_bias + i : nullptr, a.g + r * a.g_ld + a.g_col0 + i, a.Sg, a.g_stride));
+        }
+    }
+    finish_row<NV, W>(a, r, t, old, slots);
 }
 
 __global__ void __launch_bounds__(256)
@@ -271,11 +294,13 @@ extern "C" int jb_norm_residual_norm(float *x, const float *y, int Sy, long long
     const uintptr_t all = (uintptr_t)x | (uintptr_t)y | (uintptr_t)y_bias | (uintptr_t)g | (uintptr_t)g_bias | (uintptr_t)w1 |
                           (uintptr_t)b1 | (uintptr_t)scale | (uintptr_t)w2 | (uintptr_t)b2 | (uintptr_t)out;
     if (dm % 4 == 0 && dm <= 16384 && all % 16 == 0 && y_stride % 4 == 0 && (!g || (g_stride % 4 == 0 && g_ld % 4 == 0 && g_col0 % 4 == 0))) {
-        const int nv = dm <= 1024 ? 1 : dm <= 8192 ? 2 : 4;
-        const unsigned threads = (unsigned)((dm / 4 + nv * 32 - 1) / (nv * 32)) * 32;
-        launch(nv == 1 ? sublayer_norms_vec_kernel<1> : nv == 2 ? sublayer_norms_vec_kernel<2> : sublayer_norms_vec_kernel<4>,
-               (unsigned)n, threads, 0, st, a);
-        return launch_status();
+        #define JB_ROW(NV, W)                                                                          \
+    if (dm <= 128 * W * NV) {                                                                  \
+        launch(sublayer_norms_vec_kernel<NV, W>, (unsigned)n, 32 * ((dm + 128 * NV - 1) / (128 * NV)), 0, st, a); \
+        return launch_status();                                                                \
+    }
+        JB_ROW(2, 4) JB_ROW(2, 8) JB_ROW(2, 12) JB_ROW(2, 16) JB_ROW(2, 32) JB_ROW(4, 32)
+#undef JB_ROW
     }
     static unsigned long long allowed = 0;
     if (!allow_dynamic_smem(sublayer_norms_kernel, jb_norm_residual_norm_most() * 4, allowed))

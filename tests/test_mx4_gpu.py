@@ -240,7 +240,7 @@ def norm_error(t, et, w, b, eps, rms):
 @pytest.mark.parametrize("rms", [True, False])
 @pytest.mark.parametrize("gate", [False, True])
 @pytest.mark.parametrize("n,dm,S", [(1, 1, 1), (1, 32, 2), (3, 100, 1), (8, 2560, 14), (33, 1037, 3), (5, 8192, 1), (4, 9001, 2),
-                                    (200, 256, 1), (300, 2560, 1), (700, 516, 2), (2, 32768, 1), (1100, 64, 1)])
+                                    (200, 256, 1), (300, 2560, 1), (700, 516, 2), (2, 32768, 1), (1100, 64, 1), (4000, 516, 2), (1000, 2560, 1), (10000, 64, 1), (1500, 4100, 1)])
 def test_norm_residual_norm(n, dm, S, gate, rms):
     o = ops()
     x, y = rnd(n, dm, scale=3.0), rnd(S, n, dm, seed=1)
@@ -425,4 +425,19 @@ def test_linear_shared_tiles(n, m, k, launches):
     want, tol = av[some] @ wv.T, product_bound(av[some], wv, k)
     assert ((got.cpu().double()[some] - want).abs() <= tol).all()
     assert torch.equal(got, o.linear_mx4(qa, qw)) and torch.equal(got.to(BF16), o.linear_mx4(qa, qw, BF16))
+    assert o.gemm_tc_error() == 0
+
+
+@pytest.mark.parametrize("n,dm,rms", [(1000, 2560, True), (10000, 64, False), (4000, 516, True)])
+def test_norms_rows_by_themselves(n, dm, rms):
+    """A row's bits do not depend on how many rows there are."""
+    o = ops()
+    x, y, g = rnd(n, dm).to(DEV), rnd(n, dm, seed=1).to(DEV), rnd(n, dm, seed=2).to(DEV)
+    w = (1 + rnd(dm, scale=0.1)).to(DEV)
+    xs = x.clone()
+    h = o.norm_residual_norm(xs, y, w, w, 1e-5, rms, y_gate=g)
+    for rows in (slice(0, 3), slice(n - 7, n)):
+        few = x[rows].clone()
+        hf = o.norm_residual_norm(few, y[rows].clone(), w, w, 1e-5, rms, y_gate=g[rows].clone())
+        assert torch.equal(few, xs[rows]) and torch.equal(hf, h[rows])
     assert o.gemm_tc_error() == 0
