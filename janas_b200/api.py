@@ -31,6 +31,7 @@ class LLMParams:
     max_batch: int = 64         # most sequences that run together
     max_tokens: int = 0         # tokens the cache holds in all; 0: n_ctx
     device: str = "cuda:0"
+    weights: str = "stored"     # or "mx4": attention's and dense feed-forwards' matrices in 4 bits
 
 
 def params_default() -> LLMParams:
@@ -141,5 +142,5 @@ def open(path: str, params: Optional[LLMParams] = None) -> LLM:
     from .engine import Engine
     p = params or params_default()
     eng = Engine.open(path, dtype=p.dtype, max_tokens=p.max_tokens or p.n_ctx, max_seqs=p.max_batch,
-                      device=p.device, n_ctx=p.n_ctx)
+                      device=p.device, n_ctx=p.n_ctx, weights=p.weights)
     return LLM(eng, p)

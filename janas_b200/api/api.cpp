@@ -83,6 +83,7 @@ struct Opened {
     DType dtype;
     long long max_tokens;
     int max_seqs, device;
+    bool mx4;
     jb_llm_params p;
 };
 
@@ -91,6 +92,11 @@ Opened read_params(const jb_llm_params *given) {
     o.p = read_struct<jb_llm_params>(given, jb_llm_params_default);
     if (o.p.dtype != JB_LLM_BF16 && o.p.dtype != JB_LLM_F32)
         fail(JB_LLM_EINVAL, "params.dtype: JB_LLM_BF16 or JB_LLM_F32");
+    if (o.p.weights != JB_LLM_STORED && o.p.weights != JB_LLM_MX4)
+        fail(JB_LLM_EINVAL, "params.weights: JB_LLM_STORED or JB_LLM_MX4");
+    if (o.p.weights == JB_LLM_MX4 && o.p.dtype != JB_LLM_BF16)
+        fail(JB_LLM_EINVAL, "params.weights: JB_LLM_MX4 goes with JB_LLM_BF16 alone");
+    o.mx4 = o.p.weights == JB_LLM_MX4;
     if (o.p.n_ctx == 0 || o.p.max_batch == 0) fail(JB_LLM_EINVAL, "params: n_ctx and max_batch must be positive");
     o.dtype = o.p.dtype == JB_LLM_F32 ? F32 : BF16;
     o.max_tokens = o.p.max_tokens ? (long long)o.p.max_tokens : (long long)o.p.n_ctx;
@@ -129,7 +135,7 @@ int32_t jb_llm_open(const char *path, const jb_llm_params *p, jb_llm **out) {
         if (!path || !out) fail(JB_LLM_EINVAL, "jb_llm_open: path and out must be given");
         *out = nullptr;
         Opened o = read_params(p);
-        *out = wrap(Engine::open(path, o.dtype, o.max_tokens, o.max_seqs, o.device), o.p);
+        *out = wrap(Engine::open(path, o.dtype, o.max_tokens, o.max_seqs, o.device, o.mx4), o.p);
     });
 }
 
@@ -144,7 +150,7 @@ int32_t jb_llm_open_random(const char *config_json, uint64_t seed, const jb_llm_
         } catch (const JsonError &e) {
             fail(JB_LLM_EOPEN, std::string("config: not JSON (") + e.what() + ")");
         }
-        *out = wrap(Engine::open_random(cfg, seed, o.dtype, o.max_tokens, o.max_seqs, o.device), o.p);
+        *out = wrap(Engine::open_random(cfg, seed, o.dtype, o.max_tokens, o.max_seqs, o.device, o.mx4), o.p);
     });
 }
 
@@ -158,6 +164,7 @@ int32_t jb_llm_open_spec(const char *spec_json, const char *tensors_json, uint64
         spec.validate();
         std::unique_ptr<Device> dev(new Device(o.device));
         std::unique_ptr<DecoderModel> model(new DecoderModel(spec, o.dtype, dev.get()));
+        model->mx4 = o.mx4;
         if (tensors_json && *tensors_json) {
             // the caller's tensors are copied: the model owns what it runs on
             Json ts = Json::parse(tensors_json);

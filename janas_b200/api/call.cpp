@@ -17,7 +17,7 @@
 //   cache.new         {kv_specs, state_specs, max_tokens, max_seqs, dtype, device}   -> {id}   (device -1: bookkeeping only)
 //   cache.op          {id | llm, op, ...}            (the ops are in cache_op below);   cache.free {id}
 //   part.build        {role, spec, dtype, device}    -> {id};   part.free {id}
-//   part.tensors {id, prefix}, part.load {id, prefix, tensors}, part.info {id}, part.prepare {id, n_positions},
+//   part.tensors {id, prefix}, part.load {id, prefix, tensors}, part.pack {id} -> {packed}, part.info {id}, part.prepare {id, n_positions},
 //   part.kv_spec {id}, part.state_spec {id}, part.supports {id, kind}
 //   part.apply        {id, x, n, out_dtype, delta, rows}      a norm; the result is kept: part.result {id, out}
 //   part.forward      {id, ctx, h, cache}            a mixer or feed-forward -> {S, n, m}; then part.result
@@ -278,6 +278,12 @@ Json part_call(const std::string &method, const Json &a) {
         p.load(prefix, m);
         d.sync();
         return ok();
+    }
+    if (method == "part.pack") {
+        if (p.dtype != BF16) fail(JB_LLM_EINVAL, "part.pack: weights in 4 bits go with bfloat16 alone");
+        Json r = Json::object();
+        r.set("packed", (long long)p.pack_weights());
+        return r;
     }
     if (method == "part.prepare") {
         long long n = a.get("n_positions").as_int();

@@ -2,7 +2,7 @@
 
     janas-b200 <model-dir> [--prompt-tokens FILE | --tokens "1 2 3" | --prompt-len N]
                [--ctx N] [--temp T] [--top-k K] [--top-p P] [--min-p P] [--seed S]
-               [--max N] [--eos ID] [--stop ID ...] [--batch B] [--dtype bfloat16|float32]
+               [--max N] [--eos ID] [--stop ID ...] [--batch B] [--dtype bfloat16|float32] [--weights stored|mx4]
                [--stats]
     janas-b200 <model-dir> --chat [the sampling options, --ctx, --max]     (turns on standard input)
     janas-b200 <model-dir> --bench [--prompt N] [--gen N] [--rounds N] [--ctx N] [--batch B]
@@ -102,6 +102,8 @@ def main(argv=None) -> int:
     ap.add_argument("--stop", type=int, nargs="*", default=[], help="more stop tokens (up to 4)")
     ap.add_argument("--batch", type=int, default=1, help="sequences that run together")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default="stored", choices=["stored", "mx4"],
+                    help="mx4: the matrices of attention and dense feed-forwards in microscaled 4-bit floats")
     ap.add_argument("--stats", action="store_true")
     ap.add_argument("--chat", action="store_true", help="turns of token ids on standard input, "
                                                         "one a line; replies as lines of ids")
@@ -133,7 +135,7 @@ def main(argv=None) -> int:
     from . import api
     from .engine.generate import GenOptions
     need = args.ctx if not args.bench else max(args.ctx, args.prompt + args.gen)
-    params = api.LLMParams(n_ctx=need, dtype=args.dtype, max_batch=args.batch,
+    params = api.LLMParams(n_ctx=need, dtype=args.dtype, max_batch=args.batch, weights=args.weights,
                            max_tokens=(need + 63) // 64 * 64 * args.batch)
     try:
         llm = api.open(args.model, params)

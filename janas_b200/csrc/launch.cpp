@@ -642,9 +642,65 @@ static void plain_product(Device &d, const void *a, DType a_dt, const void *w, D
     check(jb_gemm_simt(a, a_dt, w, w_dt, out, n, m, k, scratch.as<float>(), 1, d.stream), what, need > 0 ? 2 : 1);
 }
 
+// A product with a weight in 4 bits of rows as floats, or (a_dt MX4) in 4 bits.
+static Stack mx4_product(Device &d, const void *a, DType a_dt, long long n, const DevTensor &w) {
+    Stack out;
+    out.S = 1;
+    out.n = n;
+    out.m = w.shape[0];
+    const int ni = as_int(n, "rows"), mi = as_int(out.m, "features"), ki = as_int(w.shape[1], "width");
+    const char *wc = (const char *)w.ptr, *ws = wc + mx4_code_bytes(mi, ki);
+    out.buf = d.pool.get(std::max<size_t>((size_t)n * (size_t)out.m * 4, 16));
+    const int rows = a_dt != MX4;
+    const long long need = jb_linear_mx4_scratch(ni, mi, ki, rows);
+    Buf scratch;
+    if (need > 0) scratch = d.pool.get((size_t)need);
+    if (rows)
+        check(jb_linear_mx4_rows(a, a_dt, wc, ws, out.data(), F32, ni, mi, ki, scratch.ptr, 1, d.stream), "linear (4 bits)");
+    else
+        check(jb_linear_mx4(a, (const char *)a + mx4_code_bytes(n, ki), wc, ws, out.data(), F32, ni, mi, ki, scratch.ptr, 1,
+                            d.stream), "linear (4 bits)");
+    count_launches(jb_linear_mx4_launches(ni, mi, ki, rows) - 1);
+    return out;
+}
+
+Stack linear_packed(Device &d, const void *a, long long n, const DevTensor &w) {
+    if (w.dt != MX4 || w.shape.size() != 2) fail(JB_LLM_EINVAL, "linear_packed: the weight is not in 4 bits");
+    return mx4_product(d, a, MX4, n, w);
+}
+
+Buf mx4_gated_unit(Device &d, const Stack &gu, UnitParams unit) {
+    if (!gu || gu.m % 2) fail(JB_LLM_EINVAL, "mx4_gated_unit: an odd width");
+    const long long ff = gu.m / 2;
+    Buf out = d.pool.get(std::max<size_t>(mx4_bytes(gu.n, ff), 16));
+    check(jb_mx4_gated_unit(gu.data(), gu.S, gu.stride(), out.ptr, (char *)out.ptr + mx4_code_bytes(gu.n, ff),
+                            as_int(gu.n, "rows"), as_int(ff, "features"), unit.alpha, unit.limit, unit.shift, d.stream),
+          "mx4_gated_unit");
+    return out;
+}
+
+Buf norm_residual_norm(Device &d, float *x, const Stack &y, const Stack *g, long long g_col0, const float *g_bias,
+                       const LnParams &post, const float *scale, const LnParams *next, bool rms, DType out_dt) {
+    if (!y || y.skip || (g && (!*g || g->n != y.n))) fail(JB_LLM_EINVAL, "norm_residual_norm: no sums, or a gate of other rows");
+    need_float(out_dt, "norm output");
+    Buf h;
+    if (next) h = d.pool.get(std::max<size_t>((size_t)y.n * (size_t)y.m * dtype_size(out_dt), 16));
+    check(jb_norm_residual_norm(x, y.data(), y.S, y.stride(), y.bias, g ? g->data() : nullptr, g ? g->S : 0, g ? g->stride() : 0,
+                                g ? as_int(g->m, "gate width") : 0, as_int(g_col0, "gate column"), g_bias, post.w, post.b,
+                                post.eps, scale, 1.0f, next ? next->w : nullptr, next ? next->b : nullptr,
+                                next ? next->eps : 0.0f, rms ? 1 : 0, h.ptr, nullptr, out_dt, as_int(y.n, "rows"),
+                                as_int(y.m, "width"), d.stream), "norm_residual_norm");
+    return h;
+}
+
 Stack linear(Device &d, const void *a, DType a_dt, long long n, long long k, const DevTensor &w,
              bool whole, bool force_simt, int splits) {
     need_float(a_dt, "activations");
+    if (w.dt == MX4) {
+        if (w.shape.size() != 2 || w.shape[1] != k)
+            fail(JB_LLM_EINVAL, "linear: the weight's rows are not as long as the activations'");
+        return mx4_product(d, a, a_dt, n, w);
+    }
     need_float(w.dt, "weight");
     if (w.shape.size() != 2 || w.shape[1] != k)
         fail(JB_LLM_EINVAL, "linear: the weight's rows are not as long as the activations'");

@@ -256,6 +256,16 @@ void rope_table(Device &d, const float *inv_freq_dev, int half, long long n_pos,
 // whole: S = 1 in every case.
 Stack linear(Device &d, const void *a, DType a_dt, long long n, long long k, const DevTensor &weight,
              bool whole = false, bool force_simt = false, int splits = 0);
+// (A weight in 4 bits, MX4: the rows are brought to 4 bits on the way, and the product comes whole.)
+// rows that come in 4 bits, codes and behind them scales (as mx4_gated_unit leaves them), . w^T: S = 1.
+Stack linear_packed(Device &d, const void *a, long long n, const DevTensor &w);
+// swiglu with its result in 4 bits, [n, ff]: codes and behind them scales.
+Buf mx4_gated_unit(Device &d, const Stack &gate_up, UnitParams unit);
+// The norms around a sublayer, csrc/sublayer_norms.cu: u = (sum y + y.bias) * sigmoid(sum g + g_bias) (g null: no gate; its
+// columns g_col0 .. g_col0 + dm - 1), x += scale * N1(u) in place (scale: float32 [dm] or null), and with `next` N2(x) in
+// out_dt.  rms: both norms without a mean.
+Buf norm_residual_norm(Device &d, float *x, const Stack &y, const Stack *g, long long g_col0, const float *g_bias,
+                       const LnParams &post, const float *scale, const LnParams *next, bool rms, DType out_dt);
 // One product per head: a [H, n, k] (one head's rows together) . w[H m, k]^T, head h
 // with rows h m .. h m + m - 1 of w.  The result: float32 [H, S, n, m].
 struct HeadStack {

@@ -11,6 +11,7 @@ size_t dtype_size(DType dt) {
         case F32: case I32: return 4;
         case BF16: case F16: return 2;
         case I64: return 8;
+        case MX4: break;        // no whole number of bytes: see mx4_bytes
     }
     return 0;
 }
@@ -22,8 +23,14 @@ const char *dtype_name(DType dt) {
         case I32: return "int32";
         case I64: return "int64";
         case F16: return "float16";
+        case MX4: return "mx4";
     }
     return "?";
+}
+
+size_t mx4_code_bytes(long long rows, long long k) { return (size_t)rows * (size_t)((k + 31) / 32) * 16; }
+size_t mx4_bytes(long long rows, long long k) {
+    return mx4_code_bytes(rows, k) + (size_t)((rows + 127) / 128) * (size_t)((k + 255) / 256) * 1024;
 }
 
 DType parse_compute_dtype(const std::string &n) {

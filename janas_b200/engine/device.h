@@ -25,8 +25,11 @@
 
 namespace jb {
 
-// element types; F32 and BF16 have the values the kernels' C interface uses
-enum DType : int { F32 = 0, BF16 = 1, I32 = 2, I64 = 3, F16 = 4 };
+// element types; F32 and BF16 have the values the kernels' C interface uses.  MX4: a matrix in microscaled 4-bit floats,
+// its codes and behind them its scales (csrc/mx4.cuh)
+enum DType : int { F32 = 0, BF16 = 1, I32 = 2, I64 = 3, F16 = 4, MX4 = 5 };
+size_t mx4_code_bytes(long long rows, long long k);
+size_t mx4_bytes(long long rows, long long k);
 size_t dtype_size(DType dt);
 const char *dtype_name(DType dt);
 DType parse_compute_dtype(const std::string &name);     // "bfloat16"/"bf16"/"float32"/"fp32"
@@ -98,7 +101,7 @@ struct DevTensor {
     DType dt = F32;
     std::vector<long long> shape;
     long long numel() const { long long n = 1; for (auto s : shape) n *= s; return n; }
-    size_t bytes() const { return (size_t)numel() * dtype_size(dt); }
+    size_t bytes() const { return dt == MX4 ? mx4_bytes(shape.at(0), shape.at(1)) : (size_t)numel() * dtype_size(dt); }
     explicit operator bool() const { return ptr != nullptr; }
 };
 

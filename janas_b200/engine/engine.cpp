@@ -25,6 +25,8 @@ Engine::Engine(std::unique_ptr<Device> d, std::unique_ptr<DecoderModel> m, long 
                int max_seqs)
     : dev(std::move(d)), model(std::move(m)), dtype(model->dtype) {
     if (!dev) fail(JB_LLM_EFAIL, "janas_b200 runs on a CUDA device only; there is no CPU path");
+    if (model->mx4 && model->packed == 0)
+        fail(JB_LLM_EMODEL, "weights in 4 bits: no part of this model takes them (attention and dense feed-forwards do)");
     if (jb_page() != PAGE)
         fail(JB_LLM_EFAIL, fmt("the kernels were built for pages of %d positions, the cache for %d",
                                jb_page(), PAGE));
@@ -56,7 +58,7 @@ Engine::~Engine() {
 
 static std::unique_ptr<Engine> make_engine(std::unique_ptr<ArchConfig> cfg, DType dtype, long long max_tokens,
                                            int max_seqs, int device, const Checkpoint *ckpt,
-                                           unsigned long long seed) {
+                                           unsigned long long seed, bool mx4) {
     ModelSpec spec = cfg->to_model_spec();
     // the configuration and the folder are read and checked before the device is touched
     if (ckpt) {
@@ -65,6 +67,7 @@ static std::unique_ptr<Engine> make_engine(std::unique_ptr<ArchConfig> cfg, DTyp
     }
     std::unique_ptr<Device> dev(new Device(device));
     std::unique_ptr<DecoderModel> model(new DecoderModel(spec, dtype, dev.get()));
+    model->mx4 = mx4;
     if (ckpt) model->load_checkpoint(*ckpt);
     else model->load_random(seed);
     std::unique_ptr<Engine> eng(new Engine(std::move(dev), std::move(model), max_tokens, max_seqs));
@@ -73,15 +76,15 @@ static std::unique_ptr<Engine> make_engine(std::unique_ptr<ArchConfig> cfg, DTyp
 }
 
 std::unique_ptr<Engine> Engine::open(const std::string &model_dir, DType dtype, long long max_tokens,
-                                     int max_seqs, int device) {
+                                     int max_seqs, int device, bool mx4) {
     std::unique_ptr<ArchConfig> cfg = config_from_dir(model_dir);
     Checkpoint ckpt(model_dir);
-    return make_engine(std::move(cfg), dtype, max_tokens, max_seqs, device, &ckpt, 0);
+    return make_engine(std::move(cfg), dtype, max_tokens, max_seqs, device, &ckpt, 0, mx4);
 }
 
 std::unique_ptr<Engine> Engine::open_random(const Json &config_json, unsigned long long seed, DType dtype,
-                                            long long max_tokens, int max_seqs, int device) {
-    return make_engine(config_from_json(config_json), dtype, max_tokens, max_seqs, device, nullptr, seed);
+                                            long long max_tokens, int max_seqs, int device, bool mx4) {
+    return make_engine(config_from_json(config_json), dtype, max_tokens, max_seqs, device, nullptr, seed, mx4);
 }
 
 // ------------------------------------------------------------- sequences
@@ -437,6 +440,8 @@ Json Engine::describe() const {
     Json o = Json::object();
     o.set("architecture", model->spec.architecture);
     o.set("dtype", dtype_name(dtype));
+    o.set("weights", model->mx4 ? "mx4" : "stored");
+    o.set("packed_matrices", (long long)model->packed);
     o.set("vocab_size", model->spec.vocab_size);
     o.set("hidden_size", model->spec.hidden_size);
     o.set("max_positions", max_positions);

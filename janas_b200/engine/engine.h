@@ -74,12 +74,13 @@ public:
 
     // Reads config.json, picks the model through the registry and loads the
     // folder's safetensors by tensor name.
+    // mx4: the layers' matrices in microscaled 4-bit floats, where their parts take them so.
     static std::unique_ptr<Engine> open(const std::string &model_dir, DType dtype, long long max_tokens,
-                                        int max_seqs, int device);
+                                        int max_seqs, int device, bool mx4 = false);
     // The same architecture lookup from a config.json given as text, with weights
     // made at random on the device.
     static std::unique_ptr<Engine> open_random(const Json &config_json, unsigned long long seed, DType dtype,
-                                               long long max_tokens, int max_seqs, int device);
+                                               long long max_tokens, int max_seqs, int device, bool mx4 = false);
 
     // sequences
     int new_sequence() { return cache->new_sequence(); }

@@ -47,10 +47,16 @@ class StepError(lib.LLMError, ValueError):
         lib.LLMError.__init__(self, lib.EINVAL, message)
 
 
-def _params(dtype, max_tokens: int, max_seqs: Optional[int], device, n_ctx: Optional[int]):
+WEIGHTS = {"stored": 0, "mx4": 1}
+
+
+def _params(dtype, max_tokens: int, max_seqs: Optional[int], device, n_ctx: Optional[int], weights: str = "stored"):
     p = lib.Params()
     lib.lib().jb_llm_params_default(ctypes.byref(p))
     p.dtype = lib.F32 if parse_dtype(dtype) == "float32" else lib.BF16
+    if weights not in WEIGHTS:
+        raise ValueError(f"weights {weights!r}: stored or mx4")
+    p.weights = WEIGHTS[weights]
     p.max_tokens = int(max_tokens)
     if max_seqs is None:
         max_seqs = max(1, min(256, (int(max_tokens) + 63) // 64))
@@ -101,10 +107,11 @@ class Engine:
     @classmethod
     def open(cls, model_dir: str, dtype="bfloat16", max_tokens: int = 4096,
              max_seqs: Optional[int] = None, device: str = "cuda:0",
-             n_ctx: Optional[int] = None) -> "Engine":
+             n_ctx: Optional[int] = None, weights: str = "stored") -> "Engine":
         """Reads config.json, picks the model through the registry and loads the
-        folder's safetensors by tensor name."""
-        p = _params(dtype, max_tokens, max_seqs, device, n_ctx)
+        folder's safetensors by tensor name.  weights "mx4": the matrices of attention and
+        dense feed-forwards in microscaled 4-bit floats (a bfloat16 model)."""
+        p = _params(dtype, max_tokens, max_seqs, device, n_ctx, weights)
         h = ctypes.c_void_p()
         lib.check(lib.lib().jb_llm_open(str(model_dir).encode(), ctypes.byref(p), ctypes.byref(h)))
         return cls(h.value)
@@ -112,10 +119,10 @@ class Engine:
     @classmethod
     def open_random(cls, config: Mapping[str, Any], seed: int = 0, dtype="bfloat16",
                     max_tokens: int = 4096, max_seqs: Optional[int] = None,
-                    device: str = "cuda:0", n_ctx: Optional[int] = None) -> "Engine":
+                    device: str = "cuda:0", n_ctx: Optional[int] = None, weights: str = "stored") -> "Engine":
         """A model of the architecture that ``config`` (a config.json as a
         dictionary) names, with weights made at random on the device."""
-        p = _params(dtype, max_tokens, max_seqs, device, n_ctx)
+        p = _params(dtype, max_tokens, max_seqs, device, n_ctx, weights)
         h = ctypes.c_void_p()
         lib.check(lib.lib().jb_llm_open_random(json.dumps(dict(config)).encode(), int(seed),
                                                ctypes.byref(p), ctypes.byref(h)))
@@ -124,10 +131,10 @@ class Engine:
     @classmethod
     def from_spec(cls, spec: ModelSpec, tensors: Optional[Mapping[str, Any]] = None, seed: int = 0,
                   dtype="float32", max_tokens: int = 4096, max_seqs: Optional[int] = None,
-                  device: str = "cuda:0") -> "Engine":
+                  device: str = "cuda:0", weights: str = "stored") -> "Engine":
         """A model put together from ``spec`` (layers of registered parts and their
         run order); ``tensors``: CUDA tensors by name (copied), else random weights."""
-        p = _params(dtype, max_tokens, max_seqs, device, None)
+        p = _params(dtype, max_tokens, max_seqs, device, None, weights)
         h = ctypes.c_void_p()
         tj = None
         keep = None

@@ -116,6 +116,10 @@ void DecoderModel::load_layer(int i, TensorMap &t) {
     if (b.feed_forward) b.feed_forward->load(n[1], t);
     if (b.post_ffn_norm) b.post_ffn_norm->load(n[5], t);
     b.load(spec.layers[(size_t)i].prefix, t);
+    if (mx4) {
+        packed += b.mixer->pack_weights();
+        if (b.feed_forward) packed += b.feed_forward->pack_weights();
+    }
 }
 
 void DecoderModel::load_checkpoint(const Checkpoint &ckpt) {

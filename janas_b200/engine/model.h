@@ -65,6 +65,10 @@ public:
     std::unique_ptr<Norm> final_norm, embedding_norm;
     DevTensor embedding, head, position_table, token_table, join;
     bool loaded = false;
+    // Whether the layers' matrices are brought to microscaled 4-bit floats as they are loaded, where their parts take them
+    // so, and how many were.
+    bool mx4 = false;
+    int packed = 0;
 
 private:
     void layer_names(int i, std::string n[6]) const;

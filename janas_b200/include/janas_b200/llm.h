@@ -45,6 +45,12 @@ extern "C" {
 #define JB_LLM_BF16 0       /* bfloat16 weights, cache and products on the tensor cores */
 #define JB_LLM_F32 1        /* the whole model in true 32-bit (no reduced-precision product) */
 
+#define JB_LLM_STORED 0     /* weights in their own type (bfloat16, or float32 where stored so) */
+#define JB_LLM_MX4 1        /* the matrices of attention and dense feed-forwards in microscaled 4-bit
+                               floats (blocks of 32 with a power of two each), brought to them when the
+                               model is opened; their products' inputs are brought to them step by step.
+                               JB_LLM_BF16 only; JB_LLM_EMODEL where no part of the model takes them. */
+
 typedef struct jb_llm jb_llm;                 /* an open model */
 typedef struct jb_llm_session jb_llm_session; /* a sequence that grows turn by turn */
 
@@ -59,7 +65,7 @@ struct jb_llm_params {
     uint32_t max_batch;  /* most sequences alive at one time (default 64) */
     int32_t dtype;       /* JB_LLM_BF16 (default) or JB_LLM_F32 */
     int32_t device;      /* CUDA device index (default 0) */
-    uint32_t reserved;
+    int32_t weights;     /* JB_LLM_STORED (default) or JB_LLM_MX4 */
     uint64_t max_tokens; /* tokens the cache holds in all, each sequence's count rounded up
                             to a multiple of 64; 0: n_ctx (default) */
 };

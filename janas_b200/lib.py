@@ -54,7 +54,7 @@ class CacheFull(LLMError):
 class Params(ctypes.Structure):
     _fields_ = [("size", ctypes.c_uint32), ("n_ctx", ctypes.c_uint32),
                 ("max_batch", ctypes.c_uint32), ("dtype", ctypes.c_int32),
-                ("device", ctypes.c_int32), ("reserved", ctypes.c_uint32),
+                ("device", ctypes.c_int32), ("weights", ctypes.c_int32),
                 ("max_tokens", ctypes.c_uint64)]
 
 

@@ -128,6 +128,10 @@ class BuiltPart:
             n: {"ptr": t.data_ptr(), "dtype": dtype_name(t.dtype), "shape": list(t.shape)}
             for n, t in keep.items()})
 
+    def pack(self) -> int:
+        """Brings the loaded matrices to microscaled 4-bit floats, where the part takes them so; how many."""
+        return self._call("pack")["packed"]
+
     def info(self) -> dict:
         return self._call("info")
 

@@ -79,6 +79,8 @@ public:
         position_->load(name(p, "position"), t);
     }
 
+    int pack_weights() override { return pack_matrix(*dev, w_qkv_) + pack_matrix(*dev, w_o_); }
+
     size_t weight_bytes() const override {
         return w_qkv_.bytes() + w_o_.bytes() + q_norm_.bytes() * (qk_norm_ ? 2 : 0);
     }

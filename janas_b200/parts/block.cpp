@@ -10,7 +10,8 @@
 // sandwich: a norm before and after each sublayer, and optionally a gate on the
 // sublayer's result, computed from the sublayer's own input:
 //     h = norm_in(x);  y = sublayer(h);  y *= sigmoid(G h + g);  x += norm_out(y)
-// for the mixer and then, where the layer has one, for the feed-forward.
+// for the mixer and then, where the layer has one, for the feed-forward; with a residual scale
+// per feature, x += s * norm_out(y).
 //
 // result_norm: no norm in front of a sublayer, one on its result alone; the sublayers read
 // the residual stream itself, optionally through a short causal convolution over time on
@@ -97,6 +98,9 @@ private:
 // true): false runs gate, norm and add as kernels of their own; token_side (optional):
 // {dim, col0, eps, names {gate, proj, norm}}: an input of the token's own after the sublayers,
 // from columns col0 .. col0 + dim - 1 of the model's token table (see token_side()).
+// mixer_scale / ffn_scale: the tensor names of the residual scales' vectors [hidden], absent or null for none.  A sublayer
+// with one ends in one kernel (csrc/sublayer_norms.cu): gate, norm, scale and add, and the next norm of the residual
+// stream where it is of the same kind; its norm must be a layer norm or an RMS norm with parameters in float32.
 class SandwichBlock : public Block {
 public:
     SandwichBlock(BlockParts p, const LayerSpec &ls, DType dt, Device *d) : Block(std::move(p)), dev_(d) {
@@ -108,6 +112,8 @@ public:
         hidden_ = bp.get("hidden_size").is_number() ? bp.get("hidden_size").as_int() : mixer_norm->size();
         if (bp.get("mixer_gate").is_string()) gate_name_[0] = bp.get("mixer_gate").as_string();
         if (bp.get("ffn_gate").is_string() && feed_forward) gate_name_[1] = bp.get("ffn_gate").as_string();
+        if (bp.get("mixer_scale").is_string()) scale_name_[0] = bp.get("mixer_scale").as_string();
+        if (bp.get("ffn_scale").is_string() && feed_forward) scale_name_[1] = bp.get("ffn_scale").as_string();
         if (bp.get("gate_bias").is_string()) bias_suffix_ = bp.get("gate_bias").as_string();
         if (bp.get("fuse").is_bool()) fuse_ = bp.get("fuse").as_bool();
         const Json &ts = bp.get("token_side");
@@ -144,6 +150,9 @@ public:
                 out.emplace_back(Part::name(prefix, gate_name_[i] + bias_suffix_),
                                  TensorSpec{{hidden_}, PARAM, false, 0.0f, 0.02f});
         }
+        for (int i = 0; i < 2; i++)
+            if (!scale_name_[i].empty())
+                out.emplace_back(Part::name(prefix, scale_name_[i]), TensorSpec{{hidden_}, PARAM, false, 0.5f, 0.1f});
         if (side_dim_ > 0) {
             out.emplace_back(Part::name(prefix, side_name_[0]), TensorSpec{{side_dim_, hidden_}, MATRIX, false});
             out.emplace_back(Part::name(prefix, side_name_[1]), TensorSpec{{hidden_, side_dim_}, MATRIX, false});
@@ -165,6 +174,15 @@ public:
                 in_part_[i] = p->take_side_rows(gate_[i]);
             }
         }
+        for (int i = 0; i < 2; i++) {
+            if (scale_name_[i].empty()) continue;
+            scale_[i] = Part::take(t, Part::name(prefix, scale_name_[i]));
+            ops::LnParams lp;
+            bool rms = false;
+            if (!(i == 0 ? post_mixer_norm : post_ffn_norm)->layer_norm(&lp, &rms))
+                fail(JB_LLM_EINVAL, "sandwich: a residual scale needs a layer norm or an RMS norm with float32 parameters "
+                                    "on the sublayer's result");
+        }
         if (side_dim_ > 0)
             for (int i = 0; i < 3; i++) side_w_[i] = Part::take(t, Part::name(prefix, side_name_[i]));
         for (auto &u : unused_) t.erase(Part::name(prefix, u.first));
@@ -172,7 +190,8 @@ public:
 
     size_t weight_bytes() const override {
         // a gate that went into its sublayer's first product is counted there
-        return gate_[0].bytes() + gate_[1].bytes() + gate_bias_[0].bytes() + gate_bias_[1].bytes() +
+        return (scale_[0] ? scale_[0].bytes() : 0) + (scale_[1] ? scale_[1].bytes() : 0) +
+               gate_[0].bytes() + gate_[1].bytes() + gate_bias_[0].bytes() + gate_bias_[1].bytes() +
                side_w_[0].bytes() + side_w_[1].bytes() + side_w_[2].bytes();
     }
 
@@ -237,6 +256,20 @@ private:
         Device &d = *ctx.dev;
         long long n = ctx.n_rows;
         const float *g_bias = gate_bias_[which] ? (const float *)gate_bias_[which].ptr : nullptr;
+        if (scale_[which]) {
+            ops::LnParams lp, ln;
+            bool rms = false, next_rms = false;
+            post->layer_norm(&lp, &rms);
+            if (y.skip) ops::resolve_bias(d, y);
+            const bool with_next = next && next->layer_norm(&ln, &next_rms) && next_rms == rms && next->size() == hidden_;
+            Buf h = ops::norm_residual_norm(d, x, y, g ? &g : nullptr, col0, g_bias, lp, (const float *)scale_[which].ptr,
+                                            with_next ? &ln : nullptr, rms, ctx.dtype);
+            if (with_next) {
+                ctx.normed = std::move(h);
+                ctx.normed_by = next;
+            }
+            return;
+        }
         ops::DytParams pp, np;
         if (fuse_ && g && post->dynamic_tanh(&pp)) {
             bool fuse_next = next && next->dynamic_tanh(&np);
@@ -307,7 +340,8 @@ private:
     std::string side_name_[3];
     DevTensor side_w_[3];
     bool fuse_ = true;      // false: every step as a kernel of its own (for comparisons)
-    std::string gate_name_[2], bias_suffix_;
+    std::string gate_name_[2], bias_suffix_, scale_name_[2];
+    DevTensor scale_[2];
     DevTensor gate_[2], gate_bias_[2];
     bool in_part_[2] = {false, false};     // the gate's rows lie in the sublayer's first product
     std::vector<std::pair<std::string, std::vector<long long>>> unused_;

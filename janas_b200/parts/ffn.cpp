@@ -61,6 +61,8 @@ public:
         w_down_ = take(t, name(prefix, n_down_));
     }
 
+    int pack_weights() override { return pack_matrix(*dev, w_gate_up_) + pack_matrix(*dev, w_down_); }
+
     size_t weight_bytes() const override { return w_gate_up_.bytes() + w_down_.bytes(); }
 
     Stack forward(StepContext &ctx, const void *h) override {
@@ -68,6 +70,12 @@ public:
         long long n = ctx.n_rows;
         Buf act;
         fused_last_ = false;
+        if (w_gate_up_.dt == MX4) {
+            Stack gu = ops::linear(d, h, ctx.dtype, n, hidden_, w_gate_up_);
+            Buf q = ops::mx4_gated_unit(d, gu, unit_);
+            gu = Stack();
+            return ops::linear_packed(d, q.ptr, n, w_down_);
+        }
         if (ctx.dtype == BF16 &&
             (n >= FUSED_FROM || (n <= FUSED_UP_TO && ops::linear_parts(n, 2 * inter_, hidden_) == 1))) {
             // enough rows, or enough features, to fill the SMs without cutting k:
@@ -131,6 +139,8 @@ public:
         coef_ = take(t, name(prefix, n_coef_));
     }
 
+    int pack_weights() override { return pack_matrix(*dev, w_up_) + pack_matrix(*dev, w_down_); }
+
     size_t weight_bytes() const override { return w_up_.bytes() + w_down_.bytes() + coef_.bytes(); }
 
     bool take_side_rows(DevTensor &m) override {
@@ -191,6 +201,8 @@ public:
         w_up_ = take(t, name(prefix, n_up_));
         w_down_ = take(t, name(prefix, n_down_));
     }
+
+    int pack_weights() override { return pack_matrix(*dev, w_up_) + pack_matrix(*dev, w_down_); }
 
     size_t weight_bytes() const override { return w_up_.bytes() + w_down_.bytes(); }
 

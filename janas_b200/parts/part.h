@@ -119,6 +119,9 @@ public:
     // and says in ctx.side_col0 where the side rows' columns start.  False (and
     // nothing taken) where the part cannot.  Called after load().
     virtual bool take_side_rows(DevTensor &m) { return false; }
+    // Brings the matrices of the part's products to microscaled 4-bit floats (JB_LLM_MX4), those that it takes in them, and
+    // says how many.  Called after load() and take_side_rows(), for a bfloat16 model.
+    virtual int pack_weights() { return 0; }
 
     PartSpec spec;
     DType dtype;
@@ -278,6 +281,8 @@ std::unique_ptr<Block> build_block(const LayerSpec &ls, DType dt, Device *dev);
 // gate, up as one: src/llm/model_attn.c:255, src/llm/model_ffn.c:349).  If their
 // dtypes differ, the widest is taken.  The sources are released as they are copied.
 DevTensor fuse_rows(Device &dev, std::vector<DevTensor> &mats);
+// w, a matrix of floats, in microscaled 4-bit floats, in place of itself.  Returns 1.
+int pack_matrix(Device &dev, DevTensor &w);
 // The same along the columns: matrices with equally many rows side by side.
 DevTensor fuse_cols(Device &dev, std::vector<DevTensor> &mats);
 

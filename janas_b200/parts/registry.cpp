@@ -1,6 +1,7 @@
 // Registries of part kinds: one name -> factory table for each role.
 #include <mutex>
 
+#include "../csrc/kernels.h"
 #include "part.h"
 
 namespace jb {
@@ -160,6 +161,19 @@ DevTensor fuse_rows(Device &dev, std::vector<DevTensor> &mats) {
     dev.sync();      // the sources are freed when the caller lets go of them
     for (auto &m : mats) m = DevTensor();
     return out;
+}
+
+int pack_matrix(Device &dev, DevTensor &w) {
+    if (w.shape.size() != 2 || (w.dt != F32 && w.dt != BF16) || w.shape[0] > 0x7fffffff || w.shape[1] > 0x7fffffff)
+        fail(JB_LLM_EINVAL, "pack_matrix: not a matrix of floats");
+    dev.make_current();
+    DevTensor out = dev.tensor(MX4, w.shape);
+    const int rows = (int)w.shape[0], k = (int)w.shape[1];
+    if (jb_mx4_quantize(w.ptr, w.dt, out.ptr, (char *)out.ptr + mx4_code_bytes(rows, k), rows, k, 0, dev.stream) != 0)
+        fail(JB_LLM_EFAIL, "pack_matrix: the kernel could not be launched");
+    dev.sync();      // the floats are freed when their last owner lets go of them
+    w = out;
+    return 1;
 }
 
 // Several matrices with equally many rows as one, columns one after the other (the down
