@@ -13,7 +13,7 @@
 // an MMA may still read.
 //
 // Up to 32 rows may come as floats: every CTA then brings its part of them to 4 bits itself (warps 2 to 9, a warp a row's
-// chunk, the next four chunks' loads in flight), which costs less than the launch of a kernel that does it once.
+// two chunks at a time), which costs less than the launch of a kernel that does it once.
 //
 // Every wait on an mbarrier has a time limit, as in gemm_tc.cu; when it runs out, the error word says which.
 #include "kernels.h"
@@ -35,7 +35,9 @@ template <int BN> struct MxCfg {
     static constexpr int SCALE_COL = BN < 32 ? 32 : BN;
     static constexpr int COLS = SCALE_COL + 16 * STAGES;
     static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */;
+    // (of the shared memory, `stages` are asked for: no more than a CTA has chunks, so that CTAs of the kernel behind this
+    // one find room on the SM before this one ends)
+    static constexpr int smem_bytes(int stages) { return stages * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */; }
 };
 
 // kind::mxf4 instruction descriptor: 4-bit A and B (bits 7-9 and 10-12 = 1), both K-major, N / 8 at bit 17, scales that
@@ -123,31 +125,121 @@ __device__ __forceinline__ void mx_fetch(const MxRows &a, size_t r, int col, flo
     }
 }
 
+constexpr int ROWS_NONE = 0, ROWS_BF16 = 1, ROWS_ANY = 2;   // as codes, as bfloat16 in whole 16-byte loads, as any floats
+
+// Sixteen bfloat16 of a lane.
+struct SixteenRows : SixteenBf16 {
+    __device__ __forceinline__ void fetch(const MxRows &a, size_t r, int col0, int lane)
+    {
+        load((const bf16 *)a.x + r * (size_t)a.k + col0 + 16 * lane, a.k - col0 - 16 * lane);
+    }
+};
+// Eight values of a lane from anywhere.
+struct AnyEight {
+    float v[8];
+    __device__ __forceinline__ void fetch(const MxRows &a, size_t r, int col0, int lane) { mx_fetch(a, r, col0 + 8 * lane, v); }
+    __device__ __forceinline__ uint2 pack(uint32_t &code) const { return make_uint2(mx4_pack_chunk(v, code), 0); }
+};
+
+// Brings this CTA's part of the rows, chunks c0 .. c0 + nc - 1, to 4 bits and into the stages.  Eight warps share the
+// (SPAN chunks, row) items; the loads of D spans are in flight.  Every warp waits for and arrives at every stage in turn,
+// whether it has an item there or not: it is then never more than one use of a stage behind, so that the parity that it
+// waits for names one phase.  Q: the most items of a span that a warp has.  False where a wait ran out.
+template <typename Values, int SPAN, int D, int Q, int BN>
+__device__ __forceinline__ bool mx_pack_rows(const MxRows &a, int rows, int c0, int nc, int stages, uint8_t *smem,
+                                             uint32_t full0, uint32_t empty0, int warp, volatile int *abort)
+{
+    static_assert(8 * Q >= BN, "items of a span");
+    constexpr int LANES = 32 / SPAN;            // lanes of a chunk
+    const int lane = threadIdx.x & 31, spans = (nc + SPAN - 1) / SPAN;
+    Values v[D][Q];
+    auto fetch = [&](int j, Values *to) {
+        const int r0 = (warp - j * rows) & 7;   // this warp's rows of span j: r0, r0 + 8, ..
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (j < spans && r0 + 8 * q < rows)
+                to[q].fetch(a, r0 + 8 * q, (c0 + j * SPAN) * MX4_CHUNK, lane);
+    };
+#pragma unroll
+    for (int d = 0; d < D; d++)
+        fetch(d, v[d]);
+    bool ok = true;
+    for (int j0 = 0; j0 < spans && ok; j0 += D) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            const int j = j0 + d, r0 = (warp - j * rows) & 7;
+            if (j >= spans || !ok)
+                continue;
+            uint2 packed[Q];
+            uint32_t code[Q];
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                if (r0 + 8 * q < rows)
+                    packed[q] = v[d][q].pack(code[q]);
+            fetch(j + D, v[d]);
+#pragma unroll
+            for (int h = 0; h < SPAN; h++) {
+                const int i = j * SPAN + h, s = i % stages;
+                if (i >= nc || !ok)
+                    continue;
+                if (i >= stages)
+                    ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / stages) & 1) ^ 1, abort, &g_gemm_mx4_error, 5));
+                if (!ok)
+                    continue;
+                uint8_t *stage = smem + s * MxCfg<BN>::STAGE_BYTES + MX_W_BYTES;
+                if (lane / LANES == h) {
+                    const int l = lane % LANES;
+#pragma unroll
+                    for (int q = 0; q < Q; q++) {
+                        const int r = r0 + 8 * q;
+                        if (r >= rows)
+                            continue;
+                        uint8_t *line = stage + r * 128, *scale = stage + MxCfg<BN>::A_BYTES + MX4_TILE + r * 16;
+                        if (SPAN == 2) {
+                            *reinterpret_cast<uint2 *>(line + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = packed[q];
+                            if ((l & 1) == 0)
+                                scale[(l >> 3) * 512 + ((l >> 1) & 3)] = (uint8_t)code[q];
+                        } else {
+                            *reinterpret_cast<uint32_t *>(line + (((l >> 2) ^ (r & 7)) << 4) + (l & 3) * 4) = packed[q].x;
+                            if ((l & 3) == 0)
+                                scale[(l >> 4) * 512 + ((l >> 2) & 3)] = (uint8_t)code[q];
+                        }
+                    }
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(full0 + 8 * s);
+            }
+        }
+    }
+    return ok;
+}
+
 // w_early: the weights were written before the kernel ahead of this one was launched, and may be read at once
-template <int BN, typename TO, bool ROWS>
+template <int BN, typename TO, int ROWS>
 __global__ void __launch_bounds__(MX_THREADS)
 gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
                 const uint8_t *w_scales, const uint8_t *a_scales, const MxRows a_rows, TO *__restrict__ out, int n, int m,
-                int chunks, int parts, int w_early)
+                int chunks, int parts, int stages, int w_early)
 {
     using Cfg = MxCfg<BN>;
-    constexpr int STAGES = Cfg::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = (uint64_t *)(smem + STAGES * Cfg::STAGE_BYTES);
-    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * STAGES + 1);
+    uint64_t *bars = (uint64_t *)(smem + stages * Cfg::STAGE_BYTES);
+    uint32_t *tmem_slot = (uint32_t *)(bars + 2 * stages + 1);
     volatile int *abort = (volatile int *)(tmem_slot + 1);
 
     const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int rank = blockIdx.x % parts, tile = blockIdx.x / parts;
     const int m0 = tile * MX_TILE_M, n0 = blockIdx.y * BN;
     const int c0 = (int)((long long)chunks * rank / parts), nc = (int)((long long)chunks * (rank + 1) / parts) - c0;
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), accum = smem_u32(bars + 2 * STAGES);
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + stages), accum = smem_u32(bars + 2 * stages);
     if (threadIdx.x == 0) {
         prefetch_tensor_map(&map_w);
         if (!ROWS)
             prefetch_tensor_map(&map_a);
-        for (int s = 0; s < STAGES; s++) {
+        for (int s = 0; s < stages; s++) {
             mbar_init(full0 + 8 * s, ROWS ? 9 : 1);        // the loads, and the warps that pack the rows
             mbar_init(empty0 + 8 * s, 1);
         }
@@ -183,7 +275,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             tma_load_2d(dst + MX_W_BYTES, &map_a, bar, (c0 + i) * (MX4_CHUNK / 2), n0);
             bulk_load(dst + MX_W_BYTES + Cfg::A_BYTES + MX4_TILE, as + (size_t)i * MX4_TILE, MX4_TILE, bar);
         };
-        const int pre = min(nc, STAGES);
+        const int pre = min(nc, stages);
         if (!w_early)
             pdl_wait();
         for (int i = 0; i < pre; i++) {
@@ -196,8 +288,8 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         for (int i = 0; i < pre && !ROWS; i++)
             load_a(i, smem_u32(smem + i * Cfg::STAGE_BYTES), full0 + 8 * i);
         for (int i = pre; i < nc; i++) {
-            const int s = i % STAGES;
-            const uint32_t ph = (i / STAGES) & 1;
+            const int s = i % stages;
+            const uint32_t ph = (i / stages) & 1;
             if (!mbar_wait(empty0 + 8 * s, ph ^ 1, abort, &g_gemm_mx4_error, 1))
                 break;
             const uint32_t dst = smem_u32(smem + s * Cfg::STAGE_BYTES), bar = full0 + 8 * s;
@@ -210,7 +302,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (*abort) {
             // the loads in flight: wait for each stage armed last, once, with the limit
             volatile int never = 0;
-            for (int s = 0; s < STAGES; s++)
+            for (int s = 0; s < stages; s++)
                 if (armed & (1u << s))
                     mbar_wait(full0 + 8 * s, (last_parity >> s) & 1, &never, &g_gemm_mx4_error, 4);
         }
@@ -227,7 +319,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             mx_stage<BN>(tmem, smem_desc_sw128(base, 16, 1024), smem_desc_sw128(base + MX_W_BYTES, 16, 1024), col, col + 8,
                          mx_scale_desc(scales), mx_scale_desc(scales + MX4_TILE), i != 0);
             tc_commit_warp(empty0 + 8 * s);
-            if (++s == STAGES) {
+            if (++s == stages) {
                 s = 0;
                 ph ^= 1;
             }
@@ -236,45 +328,10 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     } else if (warp >= 2) {
         // ------------------------------------------------------------ the accumulator
         pdl_wait();
-        if constexpr (ROWS) {
-            // item t: chunk t / groups of row (warp - 2) + 8 (t % groups)
-            constexpr int AHEAD = 4;
-            const int groups = (rows + 7) / 8, items = nc * groups;
-            float v[AHEAD][8];
-            auto fetch = [&](int t, float *to) {
-                const int i = t / groups, r = warp - 2 + 8 * (t - i * groups);
-                if (t < items && r < rows)
-                    mx_fetch(a_rows, r, (c0 + i) * MX4_CHUNK + 8 * lane, to);
-            };
-#pragma unroll
-            for (int d = 0; d < AHEAD; d++)
-                fetch(d, v[d]);
-            for (int t0 = 0; t0 < items && ok; t0 += AHEAD) {
-#pragma unroll
-                for (int d = 0; d < AHEAD; d++) {
-                    const int t = t0 + d, i = t / groups, g = t - i * groups, s = i % STAGES, r = warp - 2 + 8 * g;
-                    if (t >= items || !ok)
-                        continue;
-                    if (g == 0 && i >= STAGES)
-                        ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / STAGES) & 1) ^ 1, abort, &g_gemm_mx4_error, 5));
-                    uint8_t *stage = smem + s * Cfg::STAGE_BYTES + MX_W_BYTES;
-                    if (ok && r < rows) {
-                        uint32_t code;
-                        const uint32_t packed = mx4_pack_chunk(v[d], code);
-                        *reinterpret_cast<uint32_t *>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = packed;
-                        if ((lane & 3) == 0)
-                            stage[Cfg::A_BYTES + MX4_TILE + (lane >> 4) * 512 + r * 16 + ((lane >> 2) & 3)] = (uint8_t)code;
-                    }
-                    fetch(t + AHEAD, v[d]);
-                    if (ok && g == groups - 1) {
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0)
-                            mbar_arrive(full0 + 8 * s);
-                    }
-                }
-            }
-        }
+        if constexpr (ROWS == ROWS_BF16)
+            ok = mx_pack_rows<SixteenRows, 2, BN == 16 ? 3 : 2, BN / 8, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
+        else if constexpr (ROWS == ROWS_ANY)
+            ok = mx_pack_rows<AnyEight, 1, BN == 16 ? 3 : 2, BN / 8, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
         ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, abort, &g_gemm_mx4_error, 3));
         tc_fence_after();
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
@@ -771,16 +828,18 @@ static int launch_mx_pair(const void *ac, const void *as, const void *wc, const 
     return e;
 }
 
-// Parts of k (1, 2, 4 or 8) that a product's tiles are shared out in.
-static int mx_parts(int tiles, int chunks)
+// Parts of k (1, 2, 4 or 8) that a product's tiles are shared out in: as many as leave every part an SM of its own, and where
+// the CTAs pack floats themselves, which shorter parts shorten, two parts an SM (8 rows, 20 tiles of 16 chunks: codes 4.1 us
+// in 4 parts and 4.6 in 8, floats 5.4 and 5.2; 64 rows of codes 5.1 and 7.5).
+static int mx_parts(int tiles, int chunks, int per_sm)
 {
     int p = 1;
-    while (p < 8 && tiles * p * 2 <= 2 * sm_count() && p * 2 <= chunks)
+    while (p < 8 && tiles * p * 2 <= per_sm * sm_count() && p * 2 <= chunks)
         p *= 2;
     return p;
 }
 
-template <int BN, typename TO, bool ROWS>
+template <int BN, typename TO, int ROWS>
 static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, int n, int m, int k,
                      int w_early, cudaStream_t st)
 {
@@ -792,14 +851,19 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
         map_a = map_w;              // not used
     auto kern = gemm_mx4_kernel<BN, TO, ROWS>;
     static unsigned long long allowed = 0;
-    if (!allow_dynamic_smem(kern, Cfg::SMEM_BYTES, allowed))
+    if (!allow_dynamic_smem(kern, Cfg::smem_bytes(Cfg::STAGES), allowed))
         return JB_ELAUNCH;
     const int tiles_m = (m + MX_TILE_M - 1) / MX_TILE_M, tiles_n = (n + BN - 1) / BN, chunks = mx4_chunks(k);
     if (tiles_n > 65535)
         return JB_EINVAL;
-    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks);
-    launch_cluster(kern, dim3((unsigned)tiles_m * parts, tiles_n), MX_THREADS, Cfg::SMEM_BYTES, st, (unsigned)parts, map_w,
-                   map_a, (const uint8_t *)ws, (const uint8_t *)as, rows, out, n, m, chunks, parts, w_early);
+    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks, ROWS ? 2 : 1);
+    // (a part's sums, BN x 128 floats, lie in the stages' memory when the MMAs are done)
+    constexpr int SUMS = (BN * MX_TILE_M * 4 + Cfg::STAGE_BYTES - 1) / Cfg::STAGE_BYTES;
+    static_assert(SUMS <= Cfg::STAGES, "room for a part's sums");
+    int stages = (chunks + parts - 1) / parts;
+    stages = stages > Cfg::STAGES ? Cfg::STAGES : parts > 1 && stages < SUMS ? SUMS : stages;
+    launch_cluster(kern, dim3((unsigned)tiles_m * parts, tiles_n), MX_THREADS, Cfg::smem_bytes(stages), st, (unsigned)parts, map_w,
+                   map_a, (const uint8_t *)ws, (const uint8_t *)as, rows, out, n, m, chunks, parts, stages, w_early);
     return launch_status();
 }
 
@@ -811,16 +875,18 @@ static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, c
                   int m, int k, int w_early, cudaStream_t st)
 {
     if (rows.x)
-        return n <= 16 ? launch_mx<16, TO, true>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
-                       : launch_mx<32, TO, true>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+        return rows.is_bf16 && rows.vec ? (n <= 16 ? launch_mx<16, TO, ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
+                                                   : launch_mx<32, TO, ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st))
+                                        : (n <= 16 ? launch_mx<16, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
+                                                   : launch_mx<32, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st));
     if (n <= 16)
-        return launch_mx<16, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+        return launch_mx<16, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 32)
-        return launch_mx<32, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+        return launch_mx<32, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= 64)
-        return launch_mx<64, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+        return launch_mx<64, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     if (n <= MX_FEW)
-        return launch_mx<128, TO, false>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+        return launch_mx<128, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     return launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
 }
 

@@ -59,27 +59,6 @@ template <bool VEC> struct UnitSource {
     }
 };
 
-// Sixteen values of a lane as they are packed: floats, or bfloat16 as they lie in memory; zeros past the row's end.
-struct Sixteen {
-    float v[16];
-    __device__ __forceinline__ void load(const float *p, int left)
-    {
-        load8<float, true>(p, left, v);
-        load8<float, true>(p + 8, left - 8, v + 8);
-    }
-    __device__ __forceinline__ uint2 pack(uint32_t &code) const { return mx4_pack16(v, code); }
-};
-struct SixteenBf16 {
-    uint4 v[2];
-    __device__ __forceinline__ void load(const bf16 *p, int left)
-    {
-        const uint4 *q = reinterpret_cast<const uint4 *>(p);
-        v[0] = left > 0 ? q[0] : make_uint4(0, 0, 0, 0);
-        v[1] = left > 8 ? q[1] : make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ uint2 pack(uint32_t &code) const { return mx4_pack16(v, code); }
-};
-
 // total: n times the spans of 512 values of a row.  A warp takes U spans at a time, all read before the first is packed.
 template <typename T, typename Values, int U>
 __global__ void __launch_bounds__(256)

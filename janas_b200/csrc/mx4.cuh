@@ -172,6 +172,27 @@ __device__ __forceinline__ uint2 mx4_pack16(const uint4 *x, uint32_t &code)
     return make_uint2(mx4_pack8(x[0], inv), mx4_pack8(x[1], inv));
 }
 
+// Sixteen values of a lane as they are packed: floats, or bfloat16 as they lie in memory; zeros past the row's end.
+struct Sixteen {
+    float v[16];
+    __device__ __forceinline__ void load(const float *p, int left)
+    {
+        load8<float, true>(p, left, v);
+        load8<float, true>(p + 8, left - 8, v + 8);
+    }
+    __device__ __forceinline__ uint2 pack(uint32_t &code) const { return mx4_pack16(v, code); }
+};
+struct SixteenBf16 {
+    uint4 v[2];
+    __device__ __forceinline__ void load(const bf16 *p, int left)
+    {
+        const uint4 *q = reinterpret_cast<const uint4 *>(p);
+        v[0] = left > 0 ? q[0] : make_uint4(0, 0, 0, 0);
+        v[1] = left > 8 ? q[1] : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ uint2 pack(uint32_t &code) const { return mx4_pack16(v, code); }
+};
+
 // A lane's four values of a block that eight lanes share, in 16 bits, and the block's scale's code.
 __device__ __forceinline__ uint32_t mx4_pack4(const float4 &x, uint32_t &code)
 {

@@ -441,3 +441,16 @@ def test_norms_rows_by_themselves(n, dm, rms):
         hf = o.norm_residual_norm(few, y[rows].clone(), w, w, 1e-5, rms, y_gate=g[rows].clone())
         assert torch.equal(few, xs[rows]) and torch.equal(hf, h[rows])
     assert o.gemm_tc_error() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,m,k", [(1, 300, 30000), (5, 300, 30000), (16, 140, 26624), (20, 260, 30000), (32, 128, 30720), (3, 70, 29999)])
+def test_linear_of_few_long_rows(dtype, n, m, k):
+    """Rows packed in the product's kernel through several rounds of its stages."""
+    o, a, w, _, wv = product_case(n, m, k)
+    a = a.to(dtype)
+    av = plain_blocks(a)[2]
+    got = o.linear_mx4(a.to(DEV), o.mx4_quantize(w.to(DEV)))
+    assert ((got.cpu().double() - av @ wv.T).abs() <= product_bound(av, wv, k)).all()
+    assert torch.equal(got, o.linear_mx4(o.mx4_quantize(a.to(DEV)), o.mx4_quantize(w.to(DEV))))
+    assert o.gemm_tc_error() == 0
