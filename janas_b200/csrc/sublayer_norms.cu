@@ -184,7 +184,7 @@ __device__ __forceinline__ float4 gated4(const float4 &v, const float4 &z)
 
 // NV groups of four values a thread, at most W warps; every address at a 16-byte boundary.
 template <int NV, int W>
-__global__ void __launch_bounds__(32 * W)
+__global__ void __maxnreg__(NV == 2 ? 48 : 64)
 sublayer_norms_vec_kernel(const NormsArgs a)
 {
     __shared__ __align__(16) float slots[4][W];
