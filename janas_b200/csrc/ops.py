@@ -469,7 +469,7 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
                        next_weight: Optional[torch.Tensor], eps: float, rms: bool = True,
                        y_bias: Optional[torch.Tensor] = None, y_gate: Optional[torch.Tensor] = None, gate_col0: int = 0,
                        gate_bias: Optional[torch.Tensor] = None, scale=None, post_bias: Optional[torch.Tensor] = None,
-                       next_bias: Optional[torch.Tensor] = None, out="float32", next_eps: Optional[float] = None):
+                       next_bias: Optional[torch.Tensor] = None, out=torch.float32, next_eps: Optional[float] = None):
     """The end of a sublayer and the start of the next in one pass over the rows:
 
         u = (sum y + y_bias) * sigmoid(sum g + gate_bias);   x += scale * N1(u), in place;   h = N2(x)
@@ -477,13 +477,21 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
     y and y_gate: stacks of partial sums; the gate is columns gate_col0 .. gate_col0 + dm - 1 of y_gate, None: no
     gate.  scale: a float32 vector [dm] or a number, None: 1.  N1, N2: RMS norms, or with rms False layer norms, with
     a weight and optionally a bias (float32 [dm]); post_weight None: N1(u) = u; next_weight None: no h, None is
-    returned.  h is [n, dm] in ``out``: torch.float32, torch.bfloat16, or "mx4" for an Mx4."""
-    _need(x, "x", torch.float32, (None, None))
+    returned.  h is [n, dm] in ``out``: torch.float32, torch.bfloat16, or "mx4" for an Mx4.  Rows of up to 32,768
+    values; x must not share memory with y or y_gate."""
+    if _rows(x, "x"):
+        raise KernelError("x: float32 rows are needed")
     st = _stream_of(x, "x")
     n, dm = x.shape
-    y = stack(y)
-    _need(y, "y", torch.float32, (None, n, dm))
     here = x.get_device()
+    if not isinstance(y, torch.Tensor):
+        raise KernelError("y: a CUDA tensor is needed (there is no CPU path)")
+    deep = y.dim() == 3
+    S = y.shape[0] if deep else 1
+    if y.dtype is not _F32 or y.get_device() != here or (y.shape[1:] if deep else y.shape) != x.shape \
+            or not y.is_contiguous() or not S:
+        _need(stack(y), "y", torch.float32, (None, n, dm))
+        raise KernelError("norm_residual_norm: y needs at least one sum, on x's device")
     yb = None if y_bias is None else _vector(y_bias, "y_bias", dm, here)
     gb = None if gate_bias is None else _vector(gate_bias, "gate_bias", dm, here)
     w1 = None if post_weight is None else _vector(post_weight, "post_weight", dm, here)
@@ -497,6 +505,7 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
         mult = float(scale)
     Sg, g_ld, gate = 0, 0, None
     if y_gate is not None:
+        _need(y_gate, "y_gate", torch.float32)
         y_gate = stack(y_gate)
         _need(y_gate, "y_gate", torch.float32, (None, n, None))
         Sg, _, g_ld = y_gate.shape
@@ -507,14 +516,9 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
         raise KernelError("norm_residual_norm: a gate_bias without a gate")
     if (post_bias is not None and post_weight is None) or (next_bias is not None and next_weight is None):
         raise KernelError("norm_residual_norm: a norm's bias without its weight")
-    S = y.shape[0]
-    if not S or y.get_device() != here:
-        raise KernelError("norm_residual_norm: y needs at least one sum, on x's device")
     h = codes = scales = None
     kind = 0
-    if out == "float32":
-        out = torch.float32
-    if out != "mx4" and out not in _FLOATS:
+    if out is not _F32 and out is not _BF16 and out != "mx4":
         raise KernelError(f"norm_residual_norm: h is float32, bfloat16 or \"mx4\", not {out}")
     if next_weight is not None:
         if out == "mx4":
@@ -1340,8 +1344,9 @@ class Mx4:
         if codes.data_ptr() % 16 or scales.data_ptr() % 16 or codes.device != scales.device:
             raise KernelError("Mx4: codes and scales must lie on one device at addresses that 16 divides")
         self.rows, self.k = rows, k
-        # whether no kernel that may start before the writer's end can follow the writer
-        self.settled = True
+        # Whether a product may read the codes and scales as its weights before the kernel ahead of it has ended: only
+        # those that mx4_quantize has written behind a fence, and that nobody else can have written since.
+        self.settled = False
         self._buf = self._codes = codes
         self._scales = scales
         self._at_codes, self._at_scales = codes.data_ptr(), scales.data_ptr()
@@ -1370,6 +1375,7 @@ class Mx4:
 
     @property
     def codes(self) -> torch.Tensor:
+        self.settled = False            # (the caller may write to them)
         if self._codes is None:
             row = (self.k + 31) // 32 * 16
             self._codes = self._buf[:self.rows * row].view(self.rows, row)
@@ -1377,6 +1383,7 @@ class Mx4:
 
     @property
     def scales(self) -> torch.Tensor:
+        self.settled = False
         if self._scales is None:
             at = self.rows * ((self.k + 31) // 32 * 16)
             self._scales = self._buf[at:].view((self.rows + 127) // 128, (self.k + 255) // 256, 1024)
@@ -1384,6 +1391,7 @@ class Mx4:
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_F32, _BF16 = torch.float32, torch.bfloat16
 
 
 def _stream_of(t: torch.Tensor, name: str) -> int:
@@ -1394,27 +1402,36 @@ def _stream_of(t: torch.Tensor, name: str) -> int:
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
+def _rows(x: torch.Tensor, name: str) -> int:
+    """The kernels' number of the type of contiguous rows [n, k] of floats on a CUDA device (``_need`` says what is wrong;
+    this way round, what is right costs less)."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2 and x.is_contiguous():
+        dt = x.dtype
+        if dt is _F32:
+            return 0
+        if dt is _BF16:
+            return 1
+    _need(x, name, _FLOATS, (None, None))
+    raise KernelError(f"{name}: rows of floats are needed")
+
+
 def _vector(t: torch.Tensor, name: str, size: int, device: int) -> int:
     """The address of a contiguous float32 vector [size] on the device."""
-    if (t.__class__ not in _TENSORS and not isinstance(t, torch.Tensor)) or t.get_device() != device \
-            or t.dtype is not torch.float32 or t.dim() != 1 or t.size(0) != size or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype is not _F32 or t.dim() != 1 \
+            or t.numel() != size or not t.is_contiguous():
         raise KernelError(f"{name}: a contiguous float32 vector of {size} values on x's device is needed")
     return t.data_ptr()
-
-
-_TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4:
     """x [n, k] (float32 or bfloat16) in microscaled 4-bit floats: each block of 32 values along a row
     as 2^s times numbers of {0, 0.5, 1, 1.5, 2, 3, 4, 6} and a sign, s = floor(log2 max |x|) - 2 (at least
     -127), rounded to nearest, ties to even, at most 6.  A block with a NaN or an infinity stands for NaNs."""
-    _need(x, "x", _FLOATS, (None, None))
+    dt = _rows(x, "x")
     st = _stream_of(x, "x")
     n, k = x.shape
     q = Mx4._new(n, k, x, True)
-    _check(lib().jb_mx4_quantize(x.data_ptr(), _DT[x.dtype], q._at_codes, q._at_scales, n, k, 0, st), "mx4_quantize",
-           1 if n else 0)
+    _check(lib().jb_mx4_quantize(x.data_ptr(), dt, q._at_codes, q._at_scales, n, k, 0, st), "mx4_quantize", 1 if n else 0)
     return q
 
 
@@ -1459,12 +1476,13 @@ def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tenso
     L = lib()
     packed = a.__class__ is Mx4
     if packed:
-        if a.k != k:
-            raise KernelError(f"linear_mx4: rows of {a.k} values and a weight of {k}")
-        n, at = a.rows, a._buf
+        n, of, at = a.rows, a.k, a._buf
     else:
-        _need(a, "activations", _FLOATS, (None, k))
-        n, at = a.shape[0], a
+        dt = _rows(a, "activations")
+        n, of = a.shape
+        at = a
+    if of != k:
+        raise KernelError(f"linear_mx4: rows of {of} values and a weight of {k}")
     if at.get_device() != w._buf.get_device():
         raise KernelError("linear_mx4: the rows and the weight are on different devices")
     out = at.new_empty((n, m), dtype=out_dtype)
@@ -1479,7 +1497,7 @@ def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tenso
         code = L.jb_linear_mx4(a._at_codes, a._at_scales, w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m, k,
                                at_scratch, w.settled, st)
     else:
-        code = L.jb_linear_mx4_rows(a.data_ptr(), _DT[a.dtype], w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m,
+        code = L.jb_linear_mx4_rows(a.data_ptr(), dt, w._at_codes, w._at_scales, out.data_ptr(), _DT[out_dtype], n, m,
                                     k, at_scratch, w.settled, st)
     _check(code, "linear_mx4", launches if n and m else 0)
     return out

@@ -454,3 +454,34 @@ def test_linear_of_few_long_rows(dtype, n, m, k):
     assert ((got.cpu().double() - av @ wv.T).abs() <= product_bound(av, wv, k)).all()
     assert torch.equal(got, o.linear_mx4(o.mx4_quantize(a.to(DEV)), o.mx4_quantize(w.to(DEV))))
     assert o.gemm_tc_error() == 0
+
+
+@pytest.mark.parametrize("n", [5, 60, 300])
+def test_weights_given_as_codes(n):
+    """Codes and scales that the caller has written, right ahead of the product, in tensors of their own and in place."""
+    o = ops()
+    a, w = rnd(n, 544).to(DEV), o.mx4_quantize(rnd(400, 544, seed=1).to(DEV))
+    want = o.linear_mx4(a, w)
+    other = o.linear_mx4(a, o.mx4_quantize(rnd(400, 544, seed=2).to(DEV)))
+    codes, scales = torch.zeros_like(w.codes), torch.zeros_like(w.scales)
+    given = o.Mx4(codes, scales, 400, 544)
+    qa = o.mx4_quantize(a)
+    for _ in range(20):
+        codes.copy_(w.codes), scales.copy_(w.scales)
+        assert torch.equal(o.linear_mx4(qa, given), want)
+        codes.zero_()
+        assert not o.linear_mx4(qa, given).any()
+    v = o.mx4_quantize(rnd(400, 544, seed=2).to(DEV))
+    assert v.settled and torch.equal(o.linear_mx4(qa, v), other)
+    v.codes.copy_(w.codes), v.scales.copy_(w.scales)
+    assert not v.settled and torch.equal(o.linear_mx4(qa, v), want)
+
+
+def test_norms_refuse_other_shapes_of_sums():
+    o = ops()
+    x, w = rnd(4, 64).to(DEV), torch.ones(64, device=DEV)
+    for y in (x.view(1, 1, 4, 64), x.view(2, 2, 64), x[:, :63], x.view(-1), [1.0], x.cpu(), x.double()):
+        with pytest.raises(o.KernelError):
+            o.norm_residual_norm(x, y, w, w, 1e-5)
+    with pytest.raises(o.KernelError):
+        o.norm_residual_norm(x.bfloat16(), x, w, w, 1e-5)
