@@ -13,10 +13,10 @@
 // t / sqrt(mean(t^2) + eps) * w + b.  h is float32, bfloat16 or microscaled 4-bit floats (mx4.cuh).
 //
 // Bound by instructions and memory, and for few rows by the chain of sums.  A block per row, which stays in registers between
-// the sums, two groups of four values a thread (2,048 rows of 2,560 with a gate, from memory: 31 us; with five groups and a
-// quarter of the warps 42, with one group 37, though 8 rows then take 3.5 instead of 4.7; with each block's next row
-// prefetched into shared memory 36).  Rows that whole
-// 16-byte loads do not fit, or longer ones, stay in shared memory.
+// the sums, two groups of four values a thread (2,048 rows of 2,560 with a gate: 31 us from memory and 21 from the L2, where
+// the bytes take 14; with five groups and a quarter of the warps 42 from memory, with one group 37, though 8 rows then take
+// 3.5 instead of 4.2; with each block's next row prefetched into shared memory 36, into the L2 31).  Rows that whole 16-byte
+// loads do not fit, or longer ones, stay in shared memory.
 // How a row is shared out among the threads depends on its length alone, so its bits are the same in any batch.
 #include "kernels.h"
 #include "mx4.cuh"
@@ -30,7 +30,7 @@ struct NormsArgs {
     const float *y, *y_bias, *g, *g_bias, *w1, *b1, *scale, *w2, *b2;
     int Sy, Sg, g_ld, g_col0, rms, out_kind, dm;
     size_t y_stride, g_stride;
-    float eps1, mult, eps2;
+    float eps1, mult, eps2, inv_dm;
     void *out;
     uint8_t *scales;
 };
@@ -45,16 +45,16 @@ __device__ __forceinline__ float normed(float t, float inv, float w, const float
 __device__ __forceinline__ float added(float x, float c, float t) { return __fadd_rn(x, __fmul_rn(c, t)); }
 
 // mean (0 with rms) and 1 / sqrt(var + eps) of a row in shared memory
-__device__ __forceinline__ void row_moments(const float *row, int dm, float sum, bool rms, float eps, float *red,
+__device__ __forceinline__ void row_moments(const float *row, int dm, float inv_dm, float sum, bool rms, float eps, float *red,
                                             float &mean, float &inv)
 {
-    mean = rms ? 0.0f : block_sum(sum, red) * (1.0f / dm);
+    mean = rms ? 0.0f : block_sum(sum, red) * inv_dm;
     float sq = 0.0f;
     for (int i = threadIdx.x; i < dm; i += blockDim.x) {
         const float d = row[i] - mean;
         sq = fmaf(d, d, sq);
     }
-    inv = rsqrtf(block_sum(sq, red) * (1.0f / dm) + eps);
+    inv = rsqrtf(block_sum(sq, red) * inv_dm + eps);
 }
 
 // The sum of v over a block of at most W warps: every thread adds up all warps' sums, in order, from slots that no other sum
@@ -80,7 +80,7 @@ __device__ __forceinline__ float sum4(const float4 &v) { return (v.x + v.y) + (v
 // The norm of a row in registers: t <- (t - mean) / sqrt(var + eps) * w + b.  Values past the row's end are zeros before
 // and whatever comes out after.
 template <int NV, int W>
-__device__ __forceinline__ void norm_row(float4 *t, int dm, bool rms, float eps, const float *w, const float *b, float *slots)
+__device__ __forceinline__ void norm_row(float4 *t, int dm, float inv_dm, bool rms, float eps, const float *w, const float *b, float *slots)
 {
     float mean = 0.0f;
     if (!rms) {
@@ -88,7 +88,7 @@ __device__ __forceinline__ void norm_row(float4 *t, int dm, bool rms, float eps,
 #pragma unroll
         for (int j = 0; j < NV; j++)
             sum += sum4(t[j]);
-        mean = slot_sum<W>(sum, slots) * (1.0f / dm);
+        mean = slot_sum<W>(sum, slots) * inv_dm;
     }
     float sq = 0.0f;
 #pragma unroll
@@ -98,7 +98,7 @@ __device__ __forceinline__ void norm_row(float4 *t, int dm, bool rms, float eps,
             sq += (t[j].x * t[j].x + t[j].y * t[j].y) + (t[j].z * t[j].z + t[j].w * t[j].w);
         }
     }
-    const float inv = rsqrtf(slot_sum<W>(sq, slots + W) * (1.0f / dm) + eps);
+    const float inv = rsqrtf(slot_sum<W>(sq, slots + W) * inv_dm + eps);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = 4 * (threadIdx.x + j * blockDim.x);
@@ -136,7 +136,7 @@ __device__ __forceinline__ void finish_row(const NormsArgs &a, size_t r, float4 
     const int dm = a.dm;
     float *x = a.x + r * dm;
     if (a.w1)
-        norm_row<NV, W>(t, dm, a.rms, a.eps1, a.w1, a.b1, slots[0]);
+        norm_row<NV, W>(t, dm, a.inv_dm, a.rms, a.eps1, a.w1, a.b1, slots[0]);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = 4 * (threadIdx.x + j * blockDim.x);
@@ -149,7 +149,7 @@ __device__ __forceinline__ void finish_row(const NormsArgs &a, size_t r, float4 
     }
     if (!a.w2)
         return;
-    norm_row<NV, W>(t, dm, a.rms, a.eps2, a.w2, a.b2, slots[2]);
+    norm_row<NV, W>(t, dm, a.inv_dm, a.rms, a.eps2, a.w2, a.b2, slots[2]);
     const int blocks = (dm + 31) / 32, chunks = mx4_chunks(dm);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -231,7 +231,7 @@ sublayer_norms_kernel(const NormsArgs a)
     }
     float mean = 0.0f, inv = 1.0f;
     if (a.w1)
-        row_moments(row, dm, sum, a.rms, a.eps1, red, mean, inv);
+        row_moments(row, dm, a.inv_dm, sum, a.rms, a.eps1, red, mean, inv);
     sum = 0.0f;
     for (int i = threadIdx.x; i < dm; i += blockDim.x) {
         float v = row[i];
@@ -244,7 +244,7 @@ sublayer_norms_kernel(const NormsArgs a)
     }
     if (!a.w2)
         return;
-    row_moments(row, dm, sum, a.rms, a.eps2, red, mean, inv);
+    row_moments(row, dm, a.inv_dm, sum, a.rms, a.eps2, red, mean, inv);
     if (a.out_kind == OUT_MX4) {
         const int lane = threadIdx.x & 31, chunks = mx4_chunks(dm);
         __syncthreads();
@@ -290,7 +290,7 @@ extern "C" int jb_norm_residual_norm(float *x, const float *y, int Sy, long long
         (w2 && out_kind == OUT_MX4 && !out_scales))
         return JB_EINVAL;
     NormsArgs a{x, y, y_bias, g, g_bias, w1, b1, scale, w2, b2, Sy, Sg, g_ld, g_col0, rms, out_kind, dm,
-                (size_t)y_stride, (size_t)g_stride, eps1, mult, eps2, out, (uint8_t *)out_scales};
+                (size_t)y_stride, (size_t)g_stride, eps1, mult, eps2, 1.0f / dm, out, (uint8_t *)out_scales};
     const uintptr_t all = (uintptr_t)x | (uintptr_t)y | (uintptr_t)y_bias | (uintptr_t)g | (uintptr_t)g_bias | (uintptr_t)w1 |
                           (uintptr_t)b1 | (uintptr_t)scale | (uintptr_t)w2 | (uintptr_t)b2 | (uintptr_t)out;
     if (dm % 4 == 0 && dm <= 16384 && all % 16 == 0 && y_stride % 4 == 0 && (!g || (g_stride % 4 == 0 && g_ld % 4 == 0 && g_col0 % 4 == 0))) {
