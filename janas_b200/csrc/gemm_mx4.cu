@@ -12,7 +12,7 @@
 // the accumulator back.  A stage has its own columns of tensor memory for its scales, so nothing overwrites scales that
 // an MMA may still read.
 //
-// Up to 32 rows may come as floats: every CTA then brings its part of them to 4 bits itself (warps 2 to 9, a warp a row's
+// Few rows may come as floats: every CTA then brings its part of them to 4 bits itself (warps 2 to 9, a warp a row's
 // two chunks at a time), which costs less than the launch of a kernel that does it once.
 //
 // Every wait on an mbarrier has a time limit, as in gemm_tc.cu; when it runs out, the error word says which.
@@ -216,6 +216,60 @@ __device__ __forceinline__ bool mx_pack_rows(const MxRows &a, int rows, int c0, 
     return ok;
 }
 
+// The same for more rows than a warp's registers hold items of: the items of a span four at a time, once both of its stages
+// are free.
+template <typename Values, int SPAN, int BN>
+__device__ __forceinline__ bool mx_pack_many_rows(const MxRows &a, int rows, int c0, int nc, int stages, uint8_t *smem,
+                                                  uint32_t full0, uint32_t empty0, int warp, volatile int *abort)
+{
+    constexpr int LANES = 32 / SPAN, BATCH = 4;
+    const int lane = threadIdx.x & 31, spans = (nc + SPAN - 1) / SPAN, h = lane / LANES, l = lane % LANES;
+    for (int j = 0; j < spans; j++) {
+        const int i0 = j * SPAN, here = min(SPAN, nc - i0);
+        for (int t = 0; t < here; t++) {
+            const int i = i0 + t, s = i % stages;
+            if (i >= stages &&
+                !__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / stages) & 1) ^ 1, abort, &g_gemm_mx4_error, 5)))
+                return false;
+        }
+        uint8_t *stage = smem + (i0 + h) % stages * MxCfg<BN>::STAGE_BYTES + MX_W_BYTES;
+        for (int r0 = warp; r0 < rows; r0 += 8 * BATCH) {
+            Values v[BATCH];
+#pragma unroll
+            for (int q = 0; q < BATCH; q++)
+                if (r0 + 8 * q < rows)
+                    v[q].fetch(a, r0 + 8 * q, (c0 + i0) * MX4_CHUNK, lane);
+#pragma unroll
+            for (int q = 0; q < BATCH; q++) {
+                const int r = r0 + 8 * q;
+                if (r >= rows)
+                    continue;
+                uint32_t code;
+                const uint2 packed = v[q].pack(code);
+                if (h >= here)
+                    continue;
+                // (a line of 16 bytes of scales has four blocks of four rows, 32 apart)
+                uint8_t *line = stage + r * 128, *scale = stage + MxCfg<BN>::A_BYTES + MX4_TILE + (r & 31) * 16 + (r >> 5) * 4;
+                if (SPAN == 2) {
+                    *reinterpret_cast<uint2 *>(line + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = packed;
+                    if ((l & 1) == 0)
+                        scale[(l >> 3) * 512 + ((l >> 1) & 3)] = (uint8_t)code;
+                } else {
+                    *reinterpret_cast<uint32_t *>(line + (((l >> 2) ^ (r & 7)) << 4) + (l & 3) * 4) = packed.x;
+                    if ((l & 3) == 0)
+                        scale[(l >> 4) * 512 + ((l >> 2) & 3)] = (uint8_t)code;
+                }
+            }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0)
+            for (int t = 0; t < here; t++)
+                mbar_arrive(full0 + 8 * ((i0 + t) % stages));
+    }
+    return true;
+}
+
 // w_early: the weights were written before the kernel ahead of this one was launched, and may be read at once
 template <int BN, typename TO, int ROWS>
 __global__ void __launch_bounds__(MX_THREADS)
@@ -328,7 +382,12 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     } else if (warp >= 2) {
         // ------------------------------------------------------------ the accumulator
         pdl_wait();
-        if constexpr (ROWS == ROWS_BF16)
+        if constexpr (ROWS != ROWS_NONE && BN > 32) {
+            if constexpr (ROWS == ROWS_BF16)
+                ok = mx_pack_many_rows<SixteenRows, 2, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
+            else
+                ok = mx_pack_many_rows<AnyEight, 1, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
+        } else if constexpr (ROWS == ROWS_BF16)
             ok = mx_pack_rows<SixteenRows, 2, BN == 16 ? 3 : 2, BN / 8, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
         else if constexpr (ROWS == ROWS_ANY)
             ok = mx_pack_rows<AnyEight, 1, BN == 16 ? 3 : 2, BN / 8, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
@@ -867,27 +926,44 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
     return launch_status();
 }
 
-constexpr int MX_ROWS_MOST = 32;    // rows that the product takes as floats
 constexpr int MX_FEW = 128;         // rows up to which a product's tiles are single CTAs'
+
+// Whether the product's CTAs pack rows of floats themselves: up to 32 rows always, and up to 128 where a warp has at most 24
+// items of a row and a chunk (about 0.2 us each), which a kernel ahead costs in launching it (77 rows x 1,003 x 1,037 of
+// floats with the call 9.9 us, with a kernel ahead 15).  With many chunks a CTA it does not pay: 128 rows x 19,456 x 2,560
+// would have 160 items a warp.
+static bool mx_packs_itself(int n, int m, int k)
+{
+    if (n <= 32)
+        return true;
+    if (n > MX_FEW)
+        return false;
+    const int chunks = mx4_chunks(k), parts = mx_parts((m + MX_TILE_M - 1) / MX_TILE_M, chunks, 2);
+    return (n + 7) / 8 * (long long)((chunks + parts - 1) / parts) <= 24;
+}
+
+template <int ROWS, typename TO>
+static int few_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, int n, int m, int k,
+                  int w_early, cudaStream_t st)
+{
+    if (n <= 16)
+        return launch_mx<16, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 32)
+        return launch_mx<32, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 64)
+        return launch_mx<64, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    return launch_mx<128, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+}
 
 template <typename TO>
 static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, void *partial, int n,
                   int m, int k, int w_early, cudaStream_t st)
 {
     if (rows.x)
-        return rows.is_bf16 && rows.vec ? (n <= 16 ? launch_mx<16, TO, ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
-                                                   : launch_mx<32, TO, ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st))
-                                        : (n <= 16 ? launch_mx<16, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
-                                                   : launch_mx<32, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st));
-    if (n <= 16)
-        return launch_mx<16, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 32)
-        return launch_mx<32, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 64)
-        return launch_mx<64, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= MX_FEW)
-        return launch_mx<128, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    return launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
+        return rows.is_bf16 && rows.vec ? few_mx<ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
+                                        : few_mx<ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    return n <= MX_FEW ? few_mx<ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
+                       : launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
 }
 
 // Tiles and partial sums are counted in 32 bits.
@@ -902,16 +978,13 @@ static bool bad_product(const void *ac, const void *as, const void *wc, const vo
 
 using namespace jb;
 
-// The most rows that jb_linear_mx4_rows packs in the product's own kernel.
-extern "C" int jb_linear_mx4_rows_most(void) { return MX_ROWS_MOST; }
-
 // Bytes of scratch that a product needs, with n rows that come as codes (rows 0) or as floats (rows 1).
 extern "C" long long jb_linear_mx4_scratch(int n, int m, int k, int rows)
 {
     if (n < 1 || m < 1 || k < 1)
         return 0;
     long long bytes = n > MX_FEW ? mx_partial_bytes(mx_schedule(n, m, k)) : 0;
-    if (rows && n > MX_ROWS_MOST)
+    if (rows && !mx_packs_itself(n, m, k))
         bytes += jb_mx4_code_bytes(n, k) + jb_mx4_scale_bytes(n, k);
     return bytes;
 }
@@ -921,7 +994,7 @@ extern "C" int jb_linear_mx4_launches(int n, int m, int k, int rows)
 {
     if (n < 1 || m < 1 || k < 1)
         return 0;
-    return 1 + (rows && n > MX_ROWS_MOST) + (n > MX_FEW && mx_partial_bytes(mx_schedule(n, m, k)) > 0);
+    return 1 + (rows && !mx_packs_itself(n, m, k)) + (n > MX_FEW && mx_partial_bytes(mx_schedule(n, m, k)) > 0);
 }
 
 // out [n, m] (out_dt 0 float32, 1 bfloat16) = a [n, k] . w [m, k]^T, both as codes and scales.  scratch: see
@@ -939,7 +1012,7 @@ extern "C" int jb_linear_mx4(const void *a_codes, const void *a_scales, const vo
 }
 
 // The same with a as floats (dt 0 float32, 1 bfloat16), which are brought to 4 bits on the way: in the product's own
-// kernel for up to jb_linear_mx4_rows_most() rows, else by a kernel ahead of it, in scratch.
+// kernel for few rows, else by a kernel ahead of it, in scratch.
 extern "C" int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, const void *w_scales, void *out, int out_dt, int n,
                                   int m, int k, void *scratch, int w_early, cudaStream_t st)
 {
@@ -947,7 +1020,7 @@ extern "C" int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, co
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;
-    if (n > MX_ROWS_MOST) {
+    if (!mx_packs_itself(n, m, k)) {
         if (!scratch)
             return JB_EINVAL;
         uint8_t *codes = (uint8_t *)scratch, *scales = codes + jb_mx4_code_bytes(n, k), *rest = scales + jb_mx4_scale_bytes(n, k);

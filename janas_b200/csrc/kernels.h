@@ -174,7 +174,6 @@ int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes
                   int out_dt, int n, int m, int k, void *scratch, int w_early, cudaStream_t st);
 int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, const void *w_scales, void *out, int out_dt,
                        int n, int m, int k, void *scratch, int w_early, cudaStream_t st);
-int jb_linear_mx4_rows_most(void);
 long long jb_linear_mx4_scratch(int n, int m, int k, int rows);
 int jb_linear_mx4_launches(int n, int m, int k, int rows);
 int jb_gemm_mx4_error(void);

@@ -1460,7 +1460,7 @@ def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
-_MX4_ROWS = 32      # up to as many rows a 4-bit product needs no scratch (jb_linear_mx4_rows_most)
+_MX4_ROWS = 32      # up to as many rows a 4-bit product never needs scratch (jb_linear_mx4_scratch)
 
 
 def linear_mx4(a, w: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:

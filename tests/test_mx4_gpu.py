@@ -485,3 +485,21 @@ def test_norms_refuse_other_shapes_of_sums():
             o.norm_residual_norm(x, y, w, w, 1e-5)
     with pytest.raises(o.KernelError):
         o.norm_residual_norm(x.bfloat16(), x, w, w, 1e-5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+# (a warp's items: 16 rows of 128 by a part's chunks, of three chunks in two parts two: 32, over 24; of two chunks one: 16)
+@pytest.mark.parametrize("n,m,k,launches", [(33, 300, 512, 1), (40, 1003, 1000, 1), (64, 140, 2048, 1), (70, 200, 1024, 1),
+                                            (97, 500, 264, 1), (128, 260, 768, 2), (128, 260, 512, 1), (127, 130, 3001, 2), (128, 3000, 2560, 2)])
+def test_linear_of_some_rows(dtype, n, m, k, launches):
+    """33 to 128 rows of floats: packed in the product's kernel where its CTAs have little to pack, ahead of it otherwise."""
+    o, a, w, _, wv = product_case(n, m, k)
+    assert o.lib().jb_linear_mx4_launches(n, m, k, 1) == launches
+    a = a.to(dtype)
+    av = plain_blocks(a)[2]
+    qw = o.mx4_quantize(w.to(DEV))
+    got = o.linear_mx4(a.to(DEV), qw)
+    assert ((got.cpu().double() - av @ wv.T).abs() <= product_bound(av, wv, k)).all()
+    half = o.linear_mx4(a.to(DEV), qw, BF16)
+    assert torch.equal(half, got.to(BF16))
+    assert o.gemm_tc_error() == 0
