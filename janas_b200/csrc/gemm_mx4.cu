@@ -234,30 +234,31 @@ __device__ __forceinline__ bool mx_pack_many_rows(const MxRows &a, int rows, int
         }
         uint8_t *stage = smem + (i0 + h) % stages * MxCfg<BN>::STAGE_BYTES + MX_W_BYTES;
         for (int r0 = warp; r0 < rows; r0 += 8 * BATCH) {
+            // (no branch between a batch's items, so that their chains run side by side: past the last row it once more)
             Values v[BATCH];
+            uint2 packed[BATCH];
+            uint32_t code[BATCH];
 #pragma unroll
             for (int q = 0; q < BATCH; q++)
-                if (r0 + 8 * q < rows)
-                    v[q].fetch(a, r0 + 8 * q, (c0 + i0) * MX4_CHUNK, lane);
+                v[q].fetch(a, min(r0 + 8 * q, rows - 1), (c0 + i0) * MX4_CHUNK, lane);
+#pragma unroll
+            for (int q = 0; q < BATCH; q++)
+                packed[q] = v[q].pack(code[q]);
 #pragma unroll
             for (int q = 0; q < BATCH; q++) {
                 const int r = r0 + 8 * q;
-                if (r >= rows)
-                    continue;
-                uint32_t code;
-                const uint2 packed = v[q].pack(code);
-                if (h >= here)
+                if (r >= rows || h >= here)
                     continue;
                 // (a line of 16 bytes of scales has four blocks of four rows, 32 apart)
                 uint8_t *line = stage + r * 128, *scale = stage + MxCfg<BN>::A_BYTES + MX4_TILE + (r & 31) * 16 + (r >> 5) * 4;
                 if (SPAN == 2) {
-                    *reinterpret_cast<uint2 *>(line + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = packed;
+                    *reinterpret_cast<uint2 *>(line + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = packed[q];
                     if ((l & 1) == 0)
-                        scale[(l >> 3) * 512 + ((l >> 1) & 3)] = (uint8_t)code;
+                        scale[(l >> 3) * 512 + ((l >> 1) & 3)] = (uint8_t)code[q];
                 } else {
-                    *reinterpret_cast<uint32_t *>(line + (((l >> 2) ^ (r & 7)) << 4) + (l & 3) * 4) = packed.x;
+                    *reinterpret_cast<uint32_t *>(line + (((l >> 2) ^ (r & 7)) << 4) + (l & 3) * 4) = packed[q].x;
                     if ((l & 3) == 0)
-                        scale[(l >> 4) * 512 + ((l >> 2) & 3)] = (uint8_t)code;
+                        scale[(l >> 4) * 512 + ((l >> 2) & 3)] = (uint8_t)code[q];
                 }
             }
         }
@@ -929,8 +930,8 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
 constexpr int MX_FEW = 128;         // rows up to which a product's tiles are single CTAs'
 
 // Whether the product's CTAs pack rows of floats themselves: up to 32 rows always, and up to 128 where a warp has at most 24
-// items of a row and a chunk (about 0.2 us each), which a kernel ahead costs in launching it (77 rows x 1,003 x 1,037 of
-// floats with the call 9.9 us, with a kernel ahead 15).  With many chunks a CTA it does not pay: 128 rows x 19,456 x 2,560
+// items of a row and a chunk (0.2 us each of aligned bfloat16, 0.4 of floats at odd addresses), about what a kernel ahead costs
+// in launching it (77 rows x 1,003 x 1,037 of floats with the call 13.4 us, with a kernel ahead 15).  With many chunks a CTA it does not pay: 128 rows x 19,456 x 2,560
 // would have 160 items a warp.
 static bool mx_packs_itself(int n, int m, int k)
 {
