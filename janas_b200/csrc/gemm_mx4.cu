@@ -889,12 +889,12 @@ static int launch_mx_pair(const void *ac, const void *as, const void *wc, const 
 }
 
 // Parts of k (1, 2, 4 or 8) that a product's tiles are shared out in: as many as leave every part an SM of its own, and where
-// the CTAs pack floats themselves, which shorter parts shorten, two parts an SM (8 rows, 20 tiles of 16 chunks: codes 4.1 us
-// in 4 parts and 4.6 in 8, floats 5.4 and 5.2; 64 rows of codes 5.1 and 7.5).
-static int mx_parts(int tiles, int chunks, int per_sm)
+// the CTAs pack up to 32 rows of floats themselves, which shorter parts shorten, two parts an SM (8 rows, 20 tiles of 16
+// chunks: codes 4.1 us in 4 parts and 4.6 in 8, floats 5.4 and 5.2; 64 rows of codes 5.1 and 7.5).
+static int mx_parts(int tiles, int chunks, bool few_floats)
 {
     int p = 1;
-    while (p < 8 && tiles * p * 2 <= per_sm * sm_count() && p * 2 <= chunks)
+    while (p < 8 && tiles * p * 2 <= (few_floats ? 2 : 1) * sm_count() && p * 2 <= chunks)
         p *= 2;
     return p;
 }
@@ -916,7 +916,7 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
     const int tiles_m = (m + MX_TILE_M - 1) / MX_TILE_M, tiles_n = (n + BN - 1) / BN, chunks = mx4_chunks(k);
     if (tiles_n > 65535)
         return JB_EINVAL;
-    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks, ROWS ? 2 : 1);
+    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks, ROWS && BN <= 32);
     // (a part's sums, BN x 128 floats, lie in the stages' memory when the MMAs are done)
     constexpr int SUMS = (BN * MX_TILE_M * 4 + Cfg::STAGE_BYTES - 1) / Cfg::STAGE_BYTES;
     static_assert(SUMS <= Cfg::STAGES, "room for a part's sums");
@@ -939,7 +939,7 @@ static bool mx_packs_itself(int n, int m, int k)
         return true;
     if (n > MX_FEW)
         return false;
-    const int chunks = mx4_chunks(k), parts = mx_parts((m + MX_TILE_M - 1) / MX_TILE_M, chunks, 2);
+    const int chunks = mx4_chunks(k), parts = mx_parts((m + MX_TILE_M - 1) / MX_TILE_M, chunks, false);
     return (n + 7) / 8 * (long long)((chunks + parts - 1) / parts) <= 24;
 }
 
