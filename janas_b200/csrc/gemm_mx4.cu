@@ -12,8 +12,8 @@
 // the accumulator back.  A stage has its own columns of tensor memory for its scales, so nothing overwrites scales that
 // an MMA may still read.
 //
-// Few rows may come as floats: every CTA then brings its part of them to 4 bits itself (warps 2 to 9, a warp a row's
-// two chunks at a time), which costs less than the launch of a kernel that does it once.
+// Few rows may come as floats, in tiles of 16 or 32 rows: every CTA then brings its part of them to 4 bits itself (warps 2
+// to 9, a warp a row's two chunks at a time), which costs less than the launch of a kernel that does it once.
 //
 // Every wait on an mbarrier has a time limit, as in gemm_tc.cu; when it runs out, the error word says which.
 #include "kernels.h"
@@ -216,61 +216,6 @@ __device__ __forceinline__ bool mx_pack_rows(const MxRows &a, int rows, int c0, 
     return ok;
 }
 
-// The same for more rows than a warp's registers hold items of: the items of a span four at a time, once both of its stages
-// are free.
-template <typename Values, int SPAN, int BN>
-__device__ __forceinline__ bool mx_pack_many_rows(const MxRows &a, int rows, int c0, int nc, int stages, uint8_t *smem,
-                                                  uint32_t full0, uint32_t empty0, int warp, volatile int *abort)
-{
-    constexpr int LANES = 32 / SPAN, BATCH = 4;
-    const int lane = threadIdx.x & 31, spans = (nc + SPAN - 1) / SPAN, h = lane / LANES, l = lane % LANES;
-    for (int j = 0; j < spans; j++) {
-        const int i0 = j * SPAN, here = min(SPAN, nc - i0);
-        for (int t = 0; t < here; t++) {
-            const int i = i0 + t, s = i % stages;
-            if (i >= stages &&
-                !__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((i / stages) & 1) ^ 1, abort, &g_gemm_mx4_error, 5)))
-                return false;
-        }
-        uint8_t *stage = smem + (i0 + h) % stages * MxCfg<BN>::STAGE_BYTES + MX_W_BYTES;
-        for (int r0 = warp; r0 < rows; r0 += 8 * BATCH) {
-            // (no branch between a batch's items, so that their chains run side by side: past the last row it once more)
-            Values v[BATCH];
-            uint2 packed[BATCH];
-            uint32_t code[BATCH];
-#pragma unroll
-            for (int q = 0; q < BATCH; q++)
-                v[q].fetch(a, min(r0 + 8 * q, rows - 1), (c0 + i0) * MX4_CHUNK, lane);
-#pragma unroll
-            for (int q = 0; q < BATCH; q++)
-                packed[q] = v[q].pack(code[q]);
-#pragma unroll
-            for (int q = 0; q < BATCH; q++) {
-                const int r = r0 + 8 * q;
-                if (r >= rows || h >= here)
-                    continue;
-                // (a line of 16 bytes of scales has four blocks of four rows, 32 apart)
-                uint8_t *line = stage + r * 128, *scale = stage + MxCfg<BN>::A_BYTES + MX4_TILE + (r & 31) * 16 + (r >> 5) * 4;
-                if (SPAN == 2) {
-                    *reinterpret_cast<uint2 *>(line + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8) = packed[q];
-                    if ((l & 1) == 0)
-                        scale[(l >> 3) * 512 + ((l >> 1) & 3)] = (uint8_t)code[q];
-                } else {
-                    *reinterpret_cast<uint32_t *>(line + (((l >> 2) ^ (r & 7)) << 4) + (l & 3) * 4) = packed[q].x;
-                    if ((l & 3) == 0)
-                        scale[(l >> 4) * 512 + ((l >> 2) & 3)] = (uint8_t)code[q];
-                }
-            }
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0)
-            for (int t = 0; t < here; t++)
-                mbar_arrive(full0 + 8 * ((i0 + t) % stages));
-    }
-    return true;
-}
-
 // w_early: the weights were written before the kernel ahead of this one was launched, and may be read at once
 template <int BN, typename TO, int ROWS>
 __global__ void __launch_bounds__(MX_THREADS)
@@ -383,15 +328,12 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     } else if (warp >= 2) {
         // ------------------------------------------------------------ the accumulator
         pdl_wait();
-        if constexpr (ROWS != ROWS_NONE && BN > 32) {
-            if constexpr (ROWS == ROWS_BF16)
-                ok = mx_pack_many_rows<SixteenRows, 2, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
-            else
-                ok = mx_pack_many_rows<AnyEight, 1, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
-        } else if constexpr (ROWS == ROWS_BF16)
-            ok = mx_pack_rows<SixteenRows, 2, BN == 16 ? 3 : 2, BN / 8, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
+        const MxRows mine{(const uint8_t *)a_rows.x + (size_t)n0 * a_rows.k * (a_rows.is_bf16 ? 2 : 4), a_rows.k, a_rows.is_bf16,
+                          a_rows.vec};
+        if constexpr (ROWS == ROWS_BF16)
+            ok = mx_pack_rows<SixteenRows, 2, BN == 16 ? 3 : 2, BN / 8, BN>(mine, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
         else if constexpr (ROWS == ROWS_ANY)
-            ok = mx_pack_rows<AnyEight, 1, BN == 16 ? 3 : 2, BN / 8, BN>(a_rows, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
+            ok = mx_pack_rows<AnyEight, 1, BN == 16 ? 3 : 2, BN / 8, BN>(mine, rows, c0, nc, stages, smem, full0, empty0, warp - 2, abort);
         ok = __all_sync(0xffffffffu, mbar_wait(accum, 0, abort, &g_gemm_mx4_error, 3));
         tc_fence_after();
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
@@ -889,7 +831,7 @@ static int launch_mx_pair(const void *ac, const void *as, const void *wc, const 
 }
 
 // Parts of k (1, 2, 4 or 8) that a product's tiles are shared out in: as many as leave every part an SM of its own, and where
-// the CTAs pack up to 32 rows of floats themselves, which shorter parts shorten, two parts an SM (8 rows, 20 tiles of 16
+// the CTAs pack the rows of floats themselves, which shorter parts shorten, two parts an SM (8 rows, 20 tiles of 16
 // chunks: codes 4.1 us in 4 parts and 4.6 in 8, floats 5.4 and 5.2; 64 rows of codes 5.1 and 7.5).
 static int mx_parts(int tiles, int chunks, bool few_floats)
 {
@@ -916,7 +858,7 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
     const int tiles_m = (m + MX_TILE_M - 1) / MX_TILE_M, tiles_n = (n + BN - 1) / BN, chunks = mx4_chunks(k);
     if (tiles_n > 65535)
         return JB_EINVAL;
-    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks, ROWS && BN <= 32);
+    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks, ROWS != ROWS_NONE);
     // (a part's sums, BN x 128 floats, lie in the stages' memory when the MMAs are done)
     constexpr int SUMS = (BN * MX_TILE_M * 4 + Cfg::STAGE_BYTES - 1) / Cfg::STAGE_BYTES;
     static_assert(SUMS <= Cfg::STAGES, "room for a part's sums");
@@ -929,42 +871,51 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
 
 constexpr int MX_FEW = 128;         // rows up to which a product's tiles are single CTAs'
 
-// Whether the product's CTAs pack rows of floats themselves: up to 32 rows always, and up to 128 where a warp has at most 24
-// items of a row and a chunk (0.2 us each of aligned bfloat16, 0.4 of floats at odd addresses), about what a kernel ahead costs
-// in launching it (77 rows x 1,003 x 1,037 of floats with the call 13.4 us, with a kernel ahead 15).  With many chunks a CTA it does not pay: 128 rows x 19,456 x 2,560
-// would have 160 items a warp.
-static bool mx_packs_itself(int n, int m, int k)
+// Rows of a tile, 16 or 32, where the product's CTAs pack rows of floats themselves, or 0 where a kernel ahead does: up to 32
+// rows always, and up to 128 where a warp has at most 12 items (a row of a chunk) to pack, as each tile along m packs the
+// same rows again.  Tiles of 16 rows leave a warp the fewest; 32 where those would be over two an SM.  77 rows of floats x
+// 1,003 x 1,037 (8 parts, 2 items): 6.1 us on the device and 8.9 with the call; quantised by a call of its own before, 8.4
+// and 15.5; all rows in one tile of 128, 13.2 and 13.4.  128 x 2,560 x 1,037 (10 items): 10.5 and 11.0, by two calls 9.6
+// and 15.4.  77 x 2,560 x 4,096 (16 items, not taken): 12.4 and 13.4, by two calls 9.2 and 15.8.
+static int mx_rows_tile(int n, int m, int k)
 {
     if (n <= 32)
-        return true;
+        return n <= 16 ? 16 : 32;
     if (n > MX_FEW)
-        return false;
-    const int chunks = mx4_chunks(k), parts = mx_parts((m + MX_TILE_M - 1) / MX_TILE_M, chunks, false);
-    return (n + 7) / 8 * (long long)((chunks + parts - 1) / parts) <= 24;
-}
-
-template <int ROWS, typename TO>
-static int few_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, int n, int m, int k,
-                  int w_early, cudaStream_t st)
-{
-    if (n <= 16)
-        return launch_mx<16, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 32)
-        return launch_mx<32, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 64)
-        return launch_mx<64, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    return launch_mx<128, TO, ROWS>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+        return 0;
+    const int chunks = mx4_chunks(k), tiles_m = (m + MX_TILE_M - 1) / MX_TILE_M;
+    for (int bn = 16; bn <= 32; bn *= 2) {
+        const long long tiles = (long long)tiles_m * ((n + bn - 1) / bn);
+        if (tiles > 2 * sm_count())
+            continue;
+        const int parts = mx_parts((int)tiles, chunks, true);
+        if (bn / 8 * ((chunks + parts - 1) / parts) <= 12)
+            return bn;
+    }
+    return 0;
 }
 
 template <typename TO>
 static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, void *partial, int n,
                   int m, int k, int w_early, cudaStream_t st)
 {
-    if (rows.x)
-        return rows.is_bf16 && rows.vec ? few_mx<ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
-                                        : few_mx<ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    return n <= MX_FEW ? few_mx<ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
-                       : launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
+    if (rows.x) {
+        const bool wide = mx_rows_tile(n, m, k) == 32;
+        if (rows.is_bf16 && rows.vec)
+            return wide ? launch_mx<32, TO, ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
+                        : launch_mx<16, TO, ROWS_BF16>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+        return wide ? launch_mx<32, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
+                    : launch_mx<16, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    }
+    if (n <= 16)
+        return launch_mx<16, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 32)
+        return launch_mx<32, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    if (n <= 64)
+        return launch_mx<64, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    if (n <= MX_FEW)
+        return launch_mx<128, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    return launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
 }
 
 // Tiles and partial sums are counted in 32 bits.
@@ -985,7 +936,7 @@ extern "C" long long jb_linear_mx4_scratch(int n, int m, int k, int rows)
     if (n < 1 || m < 1 || k < 1)
         return 0;
     long long bytes = n > MX_FEW ? mx_partial_bytes(mx_schedule(n, m, k)) : 0;
-    if (rows && !mx_packs_itself(n, m, k))
+    if (rows && mx_rows_tile(n, m, k) == 0)
         bytes += jb_mx4_code_bytes(n, k) + jb_mx4_scale_bytes(n, k);
     return bytes;
 }
@@ -995,7 +946,7 @@ extern "C" int jb_linear_mx4_launches(int n, int m, int k, int rows)
 {
     if (n < 1 || m < 1 || k < 1)
         return 0;
-    return 1 + (rows && !mx_packs_itself(n, m, k)) + (n > MX_FEW && mx_partial_bytes(mx_schedule(n, m, k)) > 0);
+    return 1 + (rows && mx_rows_tile(n, m, k) == 0) + (n > MX_FEW && mx_partial_bytes(mx_schedule(n, m, k)) > 0);
 }
 
 // out [n, m] (out_dt 0 float32, 1 bfloat16) = a [n, k] . w [m, k]^T, both as codes and scales.  scratch: see
@@ -1021,7 +972,7 @@ extern "C" int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, co
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;
-    if (!mx_packs_itself(n, m, k)) {
+    if (mx_rows_tile(n, m, k) == 0) {
         if (!scratch)
             return JB_EINVAL;
         uint8_t *codes = (uint8_t *)scratch, *scales = codes + jb_mx4_code_bytes(n, k), *rest = scales + jb_mx4_scale_bytes(n, k);

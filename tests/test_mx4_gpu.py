@@ -488,9 +488,13 @@ def test_norms_refuse_other_shapes_of_sums():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-# (a warp's items: 16 rows of 128 by a part's chunks, of three chunks in two parts two: 32, over 24; of two chunks one: 16)
+# (a warp's items: an eighth of a tile's rows by a part's chunks.  128 x 260 x 768: 24 tiles of 16 rows, two parts of at most
+# 2 chunks, 4 items; 127 x 130 x 3,001: 16 tiles, eight parts of at most 2; 128 x 3,000 x 2,560: 192 tiles of 16 rows, one
+# part of 10, 20 items, over 12, and 96 of 32 rows, two parts of 5, 20 items too; 100 x 6,000 x 700: 329 tiles of 16 rows, over
+# two an SM, and 188 of 32 rows, one part of 3, 12 items)
 @pytest.mark.parametrize("n,m,k,launches", [(33, 300, 512, 1), (40, 1003, 1000, 1), (64, 140, 2048, 1), (70, 200, 1024, 1),
-                                            (97, 500, 264, 1), (128, 260, 768, 2), (128, 260, 512, 1), (127, 130, 3001, 2), (128, 3000, 2560, 2)])
+                                            (97, 500, 264, 1), (128, 260, 768, 1), (128, 260, 512, 1), (127, 130, 3001, 1), (128, 3000, 2560, 2),
+                                            (100, 6000, 700, 1)])
 def test_linear_of_some_rows(dtype, n, m, k, launches):
     """33 to 128 rows of floats: packed in the product's kernel where its CTAs have little to pack, ahead of it otherwise."""
     o, a, w, _, wv = product_case(n, m, k)
