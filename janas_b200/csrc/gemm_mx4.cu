@@ -922,7 +922,7 @@ static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, c
 static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, const void *scratch, int out_dt, int n,
                         int m, int k)
 {
-    return n < 0 || m < 0 || k < 1 || (out_dt != 0 && out_dt != 1) || ((uintptr_t)ac | (uintptr_t)as | (uintptr_t)wc |
+    return n < 0 || m < 0 || k < 1 || n > MX4_MOST || m > MX4_MOST || k > MX4_MOST || (out_dt != 0 && out_dt != 1) || ((uintptr_t)ac | (uintptr_t)as | (uintptr_t)wc |
            (uintptr_t)ws | (uintptr_t)scratch) % 16 || ((long long)n / 16 + 1) * ((long long)m / 128 + 1) > 0x3fffffff;
 }
 
@@ -933,7 +933,7 @@ using namespace jb;
 // Bytes of scratch that a product needs, with n rows that come as codes (rows 0) or as floats (rows 1).
 extern "C" long long jb_linear_mx4_scratch(int n, int m, int k, int rows)
 {
-    if (n < 1 || m < 1 || k < 1)
+    if (n < 1 || m < 1 || k < 1 || n > MX4_MOST || m > MX4_MOST || k > MX4_MOST)
         return 0;
     long long bytes = n > MX_FEW ? mx_partial_bytes(mx_schedule(n, m, k)) : 0;
     if (rows && mx_rows_tile(n, m, k) == 0)
@@ -944,7 +944,7 @@ extern "C" long long jb_linear_mx4_scratch(int n, int m, int k, int rows)
 // How many kernels such a product launches.
 extern "C" int jb_linear_mx4_launches(int n, int m, int k, int rows)
 {
-    if (n < 1 || m < 1 || k < 1)
+    if (n < 1 || m < 1 || k < 1 || n > MX4_MOST || m > MX4_MOST || k > MX4_MOST)
         return 0;
     return 1 + (rows && mx_rows_tile(n, m, k) == 0) + (n > MX_FEW && mx_partial_bytes(mx_schedule(n, m, k)) > 0);
 }

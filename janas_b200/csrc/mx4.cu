@@ -215,15 +215,20 @@ static int values(const void *codes, const void *scales, T *out, int n, int k, c
 
 using namespace jb;
 
-extern "C" long long jb_mx4_code_bytes(int rows, int k) { return rows < 0 || k < 1 ? 0 : (long long)(mx4_row_bytes(k) * (size_t)rows); }
+static bool bad_size(int n, int k) { return n < 0 || k < 1 || n > MX4_MOST || k > MX4_MOST; }
+
+extern "C" long long jb_mx4_code_bytes(int rows, int k)
+{
+    return bad_size(rows, k) ? 0 : (long long)(mx4_row_bytes(k) * (size_t)rows);
+}
 extern "C" long long jb_mx4_scale_bytes(int rows, int k)
 {
-    return rows < 0 || k < 1 ? 0 : (long long)((size_t)((rows + 127) / 128) * mx4_chunks(k) * MX4_TILE);
+    return bad_size(rows, k) ? 0 : (long long)((size_t)((rows + 127) / 128) * mx4_chunks(k) * MX4_TILE);
 }
 
 static bool bad_target(const void *codes, const void *scales, int n, int k)
 {
-    return n < 0 || k < 1 || (uintptr_t)codes % 16 != 0 || (uintptr_t)scales % 16 != 0;
+    return bad_size(n, k) || (uintptr_t)codes % 16 != 0 || (uintptr_t)scales % 16 != 0;
 }
 
 // x [n, k] -> codes and scales.  early: kernels behind this one may start before it has ended (they must then not

@@ -17,6 +17,7 @@ namespace jb {
 
 constexpr int MX4_CHUNK = 256;              // values of a row that a chunk of scales is for
 constexpr int MX4_TILE = 1024;              // its bytes, for 128 rows
+constexpr int MX4_MOST = 0x7fffff00;        // most rows, and values of a row: padded to a chunk or tile they are an int
 
 __host__ __device__ inline size_t mx4_row_bytes(int k) { return (size_t)((k + 31) / 32) * 16; }
 __host__ __device__ inline int mx4_chunks(int k) { return (k + MX4_CHUNK - 1) / MX4_CHUNK; }

@@ -489,7 +489,7 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
     deep = y.dim() == 3
     S = y.shape[0] if deep else 1
     if y.dtype is not _F32 or y.get_device() != here or (y.shape[1:] if deep else y.shape) != x.shape \
-            or not y.is_contiguous() or not S:
+            or not y.is_contiguous() or not 0 < S <= _MOST:
         _need(stack(y), "y", torch.float32, (None, n, dm))
         raise KernelError("norm_residual_norm: y needs at least one sum, on x's device")
     yb = None if y_bias is None else _vector(y_bias, "y_bias", dm, here)
@@ -509,7 +509,7 @@ def norm_residual_norm(x: torch.Tensor, y: torch.Tensor, post_weight: Optional[t
         y_gate = stack(y_gate)
         _need(y_gate, "y_gate", torch.float32, (None, n, None))
         Sg, _, g_ld = y_gate.shape
-        if Sg < 1 or gate_col0 < 0 or g_ld - gate_col0 < dm or y_gate.get_device() != here:
+        if not 0 < Sg <= _MOST or g_ld > _MOST or gate_col0 < 0 or g_ld - gate_col0 < dm or y_gate.get_device() != here:
             raise KernelError("norm_residual_norm: the gate's columns lie outside y_gate, or it is on another device")
         gate = y_gate.data_ptr()
     elif gate_bias is not None:
@@ -1325,6 +1325,11 @@ def linear_swiglu(a: torch.Tensor, gate_up: torch.Tensor, alpha: float = 1.0, li
     return out
 
 
+# most rows, and values of a row, that the kernels count (they pad them in 32 bits)
+_MOST = 0x7fffff00
+_MX4_SIZES = f"4-bit floats: rows of at least one value are needed, and at most {_MOST} of either"
+
+
 class Mx4:
     """A matrix [rows, k] in microscaled 4-bit floats, in device memory.
 
@@ -1337,8 +1342,8 @@ class Mx4:
     __slots__ = ("rows", "k", "settled", "_buf", "_codes", "_scales", "_at_codes", "_at_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int):
-        if k < 1 or rows < 0:
-            raise KernelError("Mx4: rows of at least one value are needed")
+        if not (0 < k <= _MOST and 0 <= rows <= _MOST):
+            raise KernelError(_MX4_SIZES)
         _need(codes, "codes", torch.uint8, (rows, (k + 31) // 32 * 16))
         _need(scales, "scales", torch.uint8, ((rows + 127) // 128, (k + 255) // 256, 1024))
         if codes.data_ptr() % 16 or scales.data_ptr() % 16 or codes.device != scales.device:
@@ -1354,8 +1359,8 @@ class Mx4:
     @classmethod
     def _new(cls, rows: int, k: int, like: torch.Tensor, settled: bool) -> "Mx4":
         """One allocation for both, codes first, on ``like``'s device."""
-        if k < 1:
-            raise KernelError("Mx4: rows of at least one value are needed")
+        if not (0 < k <= _MOST and rows <= _MOST):
+            raise KernelError(_MX4_SIZES)
         self = object.__new__(cls)
         n_codes = rows * ((k + 31) // 32 * 16)
         self._buf = like.new_empty(n_codes + (rows + 127) // 128 * ((k + 255) // 256) * 1024, dtype=torch.uint8)
@@ -1407,6 +1412,8 @@ def _rows(x: torch.Tensor, name: str) -> int:
     this way round, what is right costs less)."""
     if isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2 and x.is_contiguous():
         dt = x.dtype
+        if max(x.shape) > _MOST:
+            raise KernelError(f"{name}: more than {_MOST} rows, or values of a row")
         if dt is _F32:
             return 0
         if dt is _BF16:
@@ -1441,7 +1448,7 @@ def mx4_gated_unit(gate_up: torch.Tensor, alpha: float = 1.0, limit: float = 0.0
     _need(gate_up, "gate_up", torch.float32, (None, None, None))
     st = _stream_of(gate_up, "gate_up")
     S, n, two_ff = gate_up.shape
-    if two_ff % 2 or not S:
+    if two_ff % 2 or not 0 < S <= _MOST:
         raise KernelError("mx4_gated_unit: the gate_up width must be even, and at least one sum is needed")
     q = Mx4._new(n, two_ff // 2, gate_up, False)
     _check(lib().jb_mx4_gated_unit(gate_up.data_ptr(), S, n * two_ff, q._at_codes, q._at_scales, n, two_ff // 2, alpha, limit,
@@ -1451,6 +1458,8 @@ def mx4_gated_unit(gate_up: torch.Tensor, alpha: float = 1.0, limit: float = 0.0
 
 def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """What q stands for, as [rows, k] in float32 or bfloat16 (both hold every value exactly)."""
+    if q.__class__ is not Mx4:
+        raise KernelError("mx4_values: an Mx4 is needed (see mx4_quantize)")
     st = _stream_of(q._buf, "q")
     if out_dtype not in _FLOATS:
         raise KernelError(f"mx4_values: the output is float32 or bfloat16, not {out_dtype}")
