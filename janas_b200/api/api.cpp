@@ -11,15 +11,14 @@ namespace {
 
 // Reads a size-prefixed struct that may be shorter (an older caller) or longer (a
 // newer one) than this library's: the bytes both know are copied over the defaults.
-template <class T>
-T read_struct(const T *given, void (*defaults)(T *)) {
+// G: the struct by whose pointer callers pass it, T itself or what T starts with.
+template <class T, class G>
+T read_struct(const G *given, void (*defaults)(T *)) {
     T out;
     defaults(&out);
     if (given) {
         if (given->size < sizeof(uint32_t)) fail(JB_LLM_EINVAL, "a parameter struct's size field is not set");
-        size_t n = std::min<size_t>(given->size, sizeof(T));
-        memcpy(&out, given, n);
-        out.size = sizeof(T);
+        memcpy(&out, given, std::min<size_t>(given->size, sizeof(T)));
     }
     return out;
 }
@@ -89,14 +88,16 @@ struct Opened {
 
 Opened read_params(const jb_llm_params *given) {
     Opened o;
-    o.p = read_struct<jb_llm_params>(given, jb_llm_params_default);
+    const jb_llm_weight_params all = read_struct<jb_llm_weight_params>(given, jb_llm_weight_params_default);
+    o.p = all.base;
+    o.p.size = sizeof o.p;
     if (o.p.dtype != JB_LLM_BF16 && o.p.dtype != JB_LLM_F32)
         fail(JB_LLM_EINVAL, "params.dtype: JB_LLM_BF16 or JB_LLM_F32");
-    if (o.p.weights != JB_LLM_STORED && o.p.weights != JB_LLM_MX4)
+    if (all.weights != JB_LLM_STORED && all.weights != JB_LLM_MX4)
         fail(JB_LLM_EINVAL, "params.weights: JB_LLM_STORED or JB_LLM_MX4");
-    if (o.p.weights == JB_LLM_MX4 && o.p.dtype != JB_LLM_BF16)
+    if (all.weights == JB_LLM_MX4 && o.p.dtype != JB_LLM_BF16)
         fail(JB_LLM_EINVAL, "params.weights: JB_LLM_MX4 goes with JB_LLM_BF16 alone");
-    o.mx4 = o.p.weights == JB_LLM_MX4;
+    o.mx4 = all.weights == JB_LLM_MX4;
     if (o.p.n_ctx == 0 || o.p.max_batch == 0) fail(JB_LLM_EINVAL, "params: n_ctx and max_batch must be positive");
     o.dtype = o.p.dtype == JB_LLM_F32 ? F32 : BF16;
     o.max_tokens = o.p.max_tokens ? (long long)o.p.max_tokens : (long long)o.p.n_ctx;
@@ -121,6 +122,14 @@ void jb_llm_params_default(jb_llm_params *p) {
     p->dtype = JB_LLM_BF16;
     p->device = 0;
     p->max_tokens = 0;
+}
+
+void jb_llm_weight_params_default(jb_llm_weight_params *w) {
+    if (!w) return;
+    memset(w, 0, sizeof *w);
+    jb_llm_params_default(&w->base);
+    w->base.size = sizeof *w;
+    w->weights = JB_LLM_STORED;
 }
 
 void jb_gen_options_default(jb_gen_options *o) {

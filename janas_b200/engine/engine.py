@@ -52,7 +52,7 @@ WEIGHTS = {"stored": 0, "mx4": 1}
 
 def _params(dtype, max_tokens: int, max_seqs: Optional[int], device, n_ctx: Optional[int], weights: str = "stored"):
     p = lib.Params()
-    lib.lib().jb_llm_params_default(ctypes.byref(p))
+    lib.lib().jb_llm_weight_params_default(ctypes.byref(p))
     p.dtype = lib.F32 if parse_dtype(dtype) == "float32" else lib.BF16
     if weights not in WEIGHTS:
         raise ValueError(f"weights {weights!r}: stored or mx4")

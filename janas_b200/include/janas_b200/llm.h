@@ -65,11 +65,20 @@ struct jb_llm_params {
     uint32_t max_batch;  /* most sequences alive at one time (default 64) */
     int32_t dtype;       /* JB_LLM_BF16 (default) or JB_LLM_F32 */
     int32_t device;      /* CUDA device index (default 0) */
-    int32_t weights;     /* JB_LLM_STORED (default) or JB_LLM_MX4 */
+    uint32_t reserved;   /* not read */
     uint64_t max_tokens; /* tokens the cache holds in all, each sequence's count rounded up
                             to a multiple of 64; 0: n_ctx (default) */
 };
 JB_API void jb_llm_params_default(struct jb_llm_params *p);
+
+/* What a caller that chooses the weights' form passes to the functions that open a model,
+   as &w.base: base.size covers both, which jb_llm_weight_params_default sets so. */
+struct jb_llm_weight_params {
+    struct jb_llm_params base;
+    int32_t weights;     /* JB_LLM_STORED (default) or JB_LLM_MX4 */
+    uint32_t reserved;   /* not read */
+};
+JB_API void jb_llm_weight_params_default(struct jb_llm_weight_params *w);
 
 /* Opens a model folder (config.json, model.safetensors or its shards). p may be
    NULL for the defaults. */

@@ -52,10 +52,12 @@ class CacheFull(LLMError):
 
 
 class Params(ctypes.Structure):
+    # (jb_llm_weight_params: jb_llm_params and what lies behind it)
     _fields_ = [("size", ctypes.c_uint32), ("n_ctx", ctypes.c_uint32),
                 ("max_batch", ctypes.c_uint32), ("dtype", ctypes.c_int32),
-                ("device", ctypes.c_int32), ("weights", ctypes.c_int32),
-                ("max_tokens", ctypes.c_uint64)]
+                ("device", ctypes.c_int32), ("reserved", ctypes.c_uint32),
+                ("max_tokens", ctypes.c_uint64),
+                ("weights", ctypes.c_int32), ("reserved2", ctypes.c_uint32)]
 
 
 class GenOptionsC(ctypes.Structure):
@@ -95,6 +97,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "jb_llm_abi_version": (I32, []),
         "jb_llm_last_error": (ctypes.c_char_p, []),
         "jb_llm_params_default": (None, [ctypes.POINTER(Params)]),
+        "jb_llm_weight_params_default": (None, [ctypes.POINTER(Params)]),
         "jb_gen_options_default": (None, [ctypes.POINTER(GenOptionsC)]),
         "jb_llm_open": (I32, [ctypes.c_char_p, ctypes.POINTER(Params), ctypes.POINTER(P)]),
         "jb_llm_open_random": (I32, [ctypes.c_char_p, U64, ctypes.POINTER(Params),
