@@ -25,6 +25,8 @@ namespace jb {
 constexpr int MX_TILE_M = 128;
 constexpr int MX_W_BYTES = MX_TILE_M * (MX4_CHUNK / 2);
 constexpr int MX_THREADS = 320;
+constexpr int SM_SMEM = 228 * 1024, CTA_SMEM = 1024;        // an SM's shared memory, and what each CTA takes beside its own
+constexpr int SM_TMEM_COLS = 512;
 
 __device__ int g_gemm_mx4_error;    // 0, or the code of the first wait that ran out
 
@@ -33,11 +35,26 @@ template <int BN> struct MxCfg {
     static constexpr int STAGE_BYTES = MX_W_BYTES + A_BYTES + 2 * MX4_TILE;
     static constexpr int STAGES = 110 * 1024 / STAGE_BYTES > 6 ? 6 : 110 * 1024 / STAGE_BYTES;   // two CTAs fit an SM
     static constexpr int SCALE_COL = BN < 32 ? 32 : BN;
-    static constexpr int COLS = SCALE_COL + 16 * STAGES;
-    static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
-    // (of the shared memory, `stages` are asked for: no more than a CTA has chunks, so that CTAs of the kernel behind this
-    // one find room on the SM before this one ends)
-    static constexpr int smem_bytes(int stages) { return stages * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */; }
+    __host__ __device__ static constexpr int tmem_cols(int stages)
+    {
+        const int cols = SCALE_COL + 16 * stages;
+        return cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+    }
+    // Of the shared memory, `stages` are asked for: no more than a CTA has chunks, so that CTAs of the kernel behind this
+    // one find room on the SM before this one ends.  CTAs of a cluster ask for no less than their share of the SM's as their
+    // columns are of its tensor memory: a CTA that finds no columns free waits for them, while a CTA that has some keeps
+    // them until its whole cluster has its own.  Where clusters (of products on several streams) could hold more columns
+    // together than an SM has, they could wait for one another for good, and no time limit covers that wait.  So they
+    // fit an SM's tensor memory wherever they fit its shared memory.  (A CTA without a cluster waits for nobody that waits
+    // for columns: a kernel lets the one behind it start after its own CTAs have theirs.)
+    static constexpr int smem_bytes(int stages, bool cluster)
+    {
+        const int own = stages * STAGE_BYTES + 1024 /* alignment */ + 256 /* barriers */;
+        const int share = tmem_cols(stages) * (SM_SMEM / SM_TMEM_COLS) - CTA_SMEM;
+        return cluster && own < share ? share : own;
+    }
+    static constexpr int SMEM_MOST = smem_bytes(STAGES, true);
+    static_assert(SMEM_MOST <= 227 * 1024 && SCALE_COL + 16 * STAGES <= 256, "a CTA's shared memory and columns");
 };
 
 // kind::mxf4 instruction descriptor: 4-bit A and B (bits 7-9 and 10-12 = 1), both K-major, N / 8 at bit 17, scales that
@@ -249,7 +266,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::TMEM_COLS) : "memory");
+                     ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::tmem_cols(stages)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -394,7 +411,7 @@ gemm_mx4_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     __syncthreads();
     if (warp == 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-                     ::"r"(tmem), "r"((uint32_t)Cfg::TMEM_COLS) : "memory");
+                     ::"r"(tmem), "r"((uint32_t)Cfg::tmem_cols(stages)) : "memory");
 }
 
 
@@ -425,6 +442,8 @@ constexpr int MX_SLOT_COLS = 8 + 8 * MX_ROW_TILES;      // columns of tensor mem
 static_assert(MX_PAIR_N + MX_PAIR_STAGES * MX_SLOT_COLS <= 512, "tensor memory");
 constexpr int MX_PAIR_SMEM = MX_PAIR_STAGES * MX_PAIR_STAGE_BYTES + MX_GROUPS * MX_PAIR_SCALE_BYTES + 1024 /* alignment */ +
                              256 /* barriers */;
+// (a pair has all of the tensor memory: no other CTA of a cluster fits beside it, see MxCfg::smem_bytes)
+static_assert(MX_PAIR_SMEM + CTA_SMEM + MxCfg<16>::smem_bytes(1, true) + CTA_SMEM > SM_SMEM, "room beside a pair's CTA");
 
 // Tiled loads whose bytes are counted at a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
@@ -841,11 +860,32 @@ static int mx_parts(int tiles, int chunks, bool few_floats)
     return p;
 }
 
+// How a product with tiles of BN rows is launched: its parts of k, and each CTA's stages, shared memory and columns of
+// tensor memory.
+struct MxShape {
+    int tiles_m, tiles_n, parts, stages, smem, cols;
+};
+template <int BN> static MxShape mx_shape(int n, int m, int k, bool few_floats)
+{
+    using Cfg = MxCfg<BN>;
+    MxShape s;
+    const int chunks = mx4_chunks(k);
+    s.tiles_m = (m + MX_TILE_M - 1) / MX_TILE_M, s.tiles_n = (n + BN - 1) / BN;
+    s.parts = mx_parts(s.tiles_m > 0x7fffff ? 0x7fffff : s.tiles_m * s.tiles_n, chunks, few_floats);
+    // (a part's sums, BN x 128 floats, lie in the stages' memory when the MMAs are done)
+    constexpr int SUMS = (BN * MX_TILE_M * 4 + Cfg::STAGE_BYTES - 1) / Cfg::STAGE_BYTES;
+    static_assert(SUMS <= Cfg::STAGES, "room for a part's sums");
+    s.stages = (chunks + s.parts - 1) / s.parts;
+    s.stages = s.stages > Cfg::STAGES ? Cfg::STAGES : s.parts > 1 && s.stages < SUMS ? SUMS : s.stages;
+    s.smem = Cfg::smem_bytes(s.stages, s.parts > 1);
+    s.cols = Cfg::tmem_cols(s.stages);
+    return s;
+}
+
 template <int BN, typename TO, int ROWS>
 static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, int n, int m, int k,
                      int w_early, cudaStream_t st)
 {
-    using Cfg = MxCfg<BN>;
     CUtensorMap map_w, map_a;
     if (!mx_tensor_map(wc, m, k, MX_TILE_M, &map_w) || (!ROWS && !mx_tensor_map(ac, n, k, BN, &map_a)))
         return JB_EINVAL;
@@ -853,19 +893,13 @@ static int launch_mx(const void *ac, const void *as, MxRows rows, const void *wc
         map_a = map_w;              // not used
     auto kern = gemm_mx4_kernel<BN, TO, ROWS>;
     static unsigned long long allowed = 0;
-    if (!allow_dynamic_smem(kern, Cfg::smem_bytes(Cfg::STAGES), allowed))
+    if (!allow_dynamic_smem(kern, MxCfg<BN>::SMEM_MOST, allowed))
         return JB_ELAUNCH;
-    const int tiles_m = (m + MX_TILE_M - 1) / MX_TILE_M, tiles_n = (n + BN - 1) / BN, chunks = mx4_chunks(k);
-    if (tiles_n > 65535)
+    const MxShape s = mx_shape<BN>(n, m, k, ROWS != ROWS_NONE);
+    if (s.tiles_n > 65535)
         return JB_EINVAL;
-    const int parts = mx_parts(tiles_m > 0x7fffff ? 0x7fffff : tiles_m * tiles_n, chunks, ROWS != ROWS_NONE);
-    // (a part's sums, BN x 128 floats, lie in the stages' memory when the MMAs are done)
-    constexpr int SUMS = (BN * MX_TILE_M * 4 + Cfg::STAGE_BYTES - 1) / Cfg::STAGE_BYTES;
-    static_assert(SUMS <= Cfg::STAGES, "room for a part's sums");
-    int stages = (chunks + parts - 1) / parts;
-    stages = stages > Cfg::STAGES ? Cfg::STAGES : parts > 1 && stages < SUMS ? SUMS : stages;
-    launch_cluster(kern, dim3((unsigned)tiles_m * parts, tiles_n), MX_THREADS, Cfg::smem_bytes(stages), st, (unsigned)parts, map_w,
-                   map_a, (const uint8_t *)ws, (const uint8_t *)as, rows, out, n, m, chunks, parts, stages, w_early);
+    launch_cluster(kern, dim3((unsigned)s.tiles_m * s.parts, s.tiles_n), MX_THREADS, s.smem, st, (unsigned)s.parts, map_w, map_a,
+                   (const uint8_t *)ws, (const uint8_t *)as, rows, out, n, m, mx4_chunks(k), s.parts, s.stages, w_early);
     return launch_status();
 }
 
@@ -895,6 +929,9 @@ static int mx_rows_tile(int n, int m, int k)
     return 0;
 }
 
+// Rows of a tile where they come as codes, or 0: pairs' tiles.
+static int mx_codes_tile(int n) { return n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : n <= MX_FEW ? 128 : 0; }
+
 template <typename TO>
 static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, const void *ws, TO *out, void *partial, int n,
                   int m, int k, int w_early, cudaStream_t st)
@@ -907,14 +944,12 @@ static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, c
         return wide ? launch_mx<32, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st)
                     : launch_mx<16, TO, ROWS_ANY>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
     }
-    if (n <= 16)
-        return launch_mx<16, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 32)
-        return launch_mx<32, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= 64)
-        return launch_mx<64, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
-    if (n <= MX_FEW)
-        return launch_mx<128, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    switch (mx_codes_tile(n)) {
+    case 16: return launch_mx<16, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    case 32: return launch_mx<32, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    case 64: return launch_mx<64, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    case 128: return launch_mx<128, TO, ROWS_NONE>(ac, as, rows, wc, ws, out, n, m, k, w_early, st);
+    }
     return launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
 }
 
@@ -947,6 +982,20 @@ extern "C" int jb_linear_mx4_launches(int n, int m, int k, int rows)
     if (n < 1 || m < 1 || k < 1 || n > MX4_MOST || m > MX4_MOST || k > MX4_MOST)
         return 0;
     return 1 + (rows && mx_rows_tile(n, m, k) == 0) + (n > MX_FEW && mx_partial_bytes(mx_schedule(n, m, k)) > 0);
+}
+
+// How such a product's CTAs share an SM: out = {CTAs of a cluster, shared memory of a CTA in bytes, its columns of tensor
+// memory}.
+extern "C" int jb_linear_mx4_cta(int n, int m, int k, int rows, int *out)
+{
+    if (n < 1 || m < 1 || k < 1 || n > MX4_MOST || m > MX4_MOST || k > MX4_MOST)
+        return JB_EINVAL;
+    const int own = rows ? mx_rows_tile(n, m, k) : 0, tile = own ? own : mx_codes_tile(n);
+    const MxShape s = tile == 16 ? mx_shape<16>(n, m, k, own) : tile == 32 ? mx_shape<32>(n, m, k, own)
+                    : tile == 64 ? mx_shape<64>(n, m, k, false) : tile == 128 ? mx_shape<128>(n, m, k, false)
+                                 : MxShape{0, 0, 2, 0, MX_PAIR_SMEM, SM_TMEM_COLS};
+    out[0] = s.parts, out[1] = s.smem, out[2] = s.cols;
+    return JB_OK;
 }
 
 // out [n, m] (out_dt 0 float32, 1 bfloat16) = a [n, k] . w [m, k]^T, both as codes and scales.  scratch: see

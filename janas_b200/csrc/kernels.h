@@ -176,6 +176,7 @@ int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, const void *w
                        int n, int m, int k, void *scratch, int w_early, cudaStream_t st);
 long long jb_linear_mx4_scratch(int n, int m, int k, int rows);
 int jb_linear_mx4_launches(int n, int m, int k, int rows);
+int jb_linear_mx4_cta(int n, int m, int k, int rows, int *out);
 int jb_gemm_mx4_error(void);
 int jb_short_conv(const float *x, const float *w, float *state, long long slot_stride, const int32_t *row_pos,
                   const int32_t *row_seq, const int32_t *seq_slot, void *out, int out_dt, int n,
