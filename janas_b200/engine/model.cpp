@@ -115,11 +115,12 @@ void DecoderModel::load_layer(int i, TensorMap &t) {
     if (b.ffn_norm) b.ffn_norm->load(n[3], t);
     if (b.feed_forward) b.feed_forward->load(n[1], t);
     if (b.post_ffn_norm) b.post_ffn_norm->load(n[5], t);
-    b.load(spec.layers[(size_t)i].prefix, t);
+    // before the block's own tensors: a gate does not go into a matrix in 4 bits
     if (mx4) {
         packed += b.mixer->pack_weights();
         if (b.feed_forward) packed += b.feed_forward->pack_weights();
     }
+    b.load(spec.layers[(size_t)i].prefix, t);
 }
 
 void DecoderModel::load_checkpoint(const Checkpoint &ckpt) {

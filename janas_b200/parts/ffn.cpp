@@ -144,7 +144,7 @@ public:
     size_t weight_bytes() const override { return w_up_.bytes() + w_down_.bytes() + coef_.bytes(); }
 
     bool take_side_rows(DevTensor &m) override {
-        if (!w_up_ || m.shape.size() != 2 || m.shape[1] != hidden_ || side_) return false;
+        if (!w_up_ || w_up_.dt == MX4 || m.shape.size() != 2 || m.shape[1] != hidden_ || side_) return false;
         std::vector<DevTensor> both = {w_up_, m};
         w_up_ = DevTensor();
         m = DevTensor();

@@ -120,7 +120,8 @@ public:
     // nothing taken) where the part cannot.  Called after load().
     virtual bool take_side_rows(DevTensor &m) { return false; }
     // Brings the matrices of the part's products to microscaled 4-bit floats (JB_LLM_MX4), those that it takes in them, and
-    // says how many.  Called after load() and take_side_rows(), for a bfloat16 model.
+    // says how many.  Called after load() and before take_side_rows(), for a bfloat16 model: side rows stay as they are, so
+    // a packed matrix takes none.
     virtual int pack_weights() { return 0; }
 
     PartSpec spec;
