@@ -100,7 +100,8 @@ private:
 // from columns col0 .. col0 + dim - 1 of the model's token table (see token_side()).
 // mixer_scale / ffn_scale: the tensor names of the residual scales' vectors [hidden], absent or null for none.  A sublayer
 // with one ends in one kernel (csrc/sublayer_norms.cu): gate, norm, scale and add, and the next norm of the residual
-// stream where it is of the same kind; its norm must be a layer norm or an RMS norm with parameters in float32.
+// stream where it is of the same kind (fuse false: gate, norm, and scale and add, a kernel each); its norm must be a layer
+// norm or an RMS norm with parameters in float32.
 class SandwichBlock : public Block {
 public:
     SandwichBlock(BlockParts p, const LayerSpec &ls, DType dt, Device *d) : Block(std::move(p)), dev_(d) {
@@ -256,7 +257,7 @@ private:
         Device &d = *ctx.dev;
         long long n = ctx.n_rows;
         const float *g_bias = gate_bias_[which] ? (const float *)gate_bias_[which].ptr : nullptr;
-        if (scale_[which]) {
+        if (scale_[which] && fuse_) {
             ops::LnParams lp, ln;
             bool rms = false, next_rms = false;
             post->layer_norm(&lp, &rms);
@@ -287,7 +288,7 @@ private:
             ops::norm_residual_(d, x, y, lp, rms, ctx.kind == DECODE && ctx.dtype == BF16);
             return;
         }
-        // the steps one by one, for any norm: gate, norm of the result, add
+        // the steps one by one, for any norm: gate, norm of the result, (scale and) add
         Buf t;
         Stack one;
         if (g) {
@@ -301,7 +302,11 @@ private:
         one.S = 1;
         one.n = n;
         one.m = hidden_;
-        ops::add_(d, x, n, hidden_, one);
+        if (scale_[which])
+            ops::norm_residual_norm(d, x, one, nullptr, 0, nullptr, ops::LnParams(), (const float *)scale_[which].ptr, nullptr,
+                                    false, ctx.dtype);
+        else
+            ops::add_(d, x, n, hidden_, one);
     }
 
     // The token's own input to the layer, after the sublayers: with e = the token's row of the

@@ -142,3 +142,28 @@ def test_zuzelorn_in_4_bits(name):
                             dtype="bfloat16", max_tokens=1024, weights="mx4")
     assert np.array_equal(got, logits(same, toks)) and np.isfinite(got).all()
     same.close()
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("gates", [False, True])
+def test_residual_scales_step_by_step(kind, gates):
+    """fuse false: gate, norm, and scale and add, each a kernel of its own.  Each way is off from the sublayers in 64 bits
+    by at most 10 x 160 roundings a sublayer (products over up to 160 values, norms that can make their error ten times as
+    much of the result), four sublayers; so the two differ by twice that at most."""
+    from helpers import rel_err
+    from janas_b200 import lib
+    got, count = {}, {}
+    for fuse in (True, False):
+        spec = sandwich("swiglu", kind, gates, scales=True, fuse=fuse)
+        e = opened(spec, weights_of(spec), weights="stored", dtype="float32")
+        logits(e, TOKENS)
+        at = lib.call("llm.launches")["launches"]
+        got[fuse] = logits(e, TOKENS)
+        count[fuse] = lib.call("llm.launches")["launches"] - at
+        tail = logits(e, TOKENS, 5)
+        assert rel_err(tail, got[fuse]) <= 2 * 10 * 160 * 4 * torch.finfo(torch.float32).eps / 2
+        e.close()
+    # a step's kernels: a norm for each of the four sublayers' results, three norms that wait for the next sublayer (the
+    # last one the model's), and with gates four gates
+    assert count[False] > count[True] + 4
+    assert rel_err(got[False], got[True]) <= 2 * 10 * 160 * 4 * torch.finfo(torch.float32).eps / 2
