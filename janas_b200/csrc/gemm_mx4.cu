@@ -953,12 +953,13 @@ static int any_mx(const void *ac, const void *as, MxRows rows, const void *wc, c
     return launch_mx_pair<TO>(ac, as, wc, ws, out, partial, n, m, k, w_early, st);
 }
 
-// Tiles and partial sums are counted in 32 bits.
-static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, const void *scratch, int out_dt, int n,
-                        int m, int k)
+// Tiles and partial sums are counted in 32 bits; every address is one that 16 divides.
+static bool bad_product(const void *ac, const void *as, const void *wc, const void *ws, const void *out, const void *scratch,
+                        int out_dt, int n, int m, int k)
 {
-    return n < 0 || m < 0 || k < 1 || n > MX4_MOST || m > MX4_MOST || k > MX4_MOST || (out_dt != 0 && out_dt != 1) || ((uintptr_t)ac | (uintptr_t)as | (uintptr_t)wc |
-           (uintptr_t)ws | (uintptr_t)scratch) % 16 || ((long long)n / 16 + 1) * ((long long)m / 128 + 1) > 0x3fffffff;
+    return n < 0 || m < 0 || k < 1 || n > MX4_MOST || m > MX4_MOST || k > MX4_MOST || (out_dt != 0 && out_dt != 1) ||
+           ((uintptr_t)ac | (uintptr_t)as | (uintptr_t)wc | (uintptr_t)ws | (uintptr_t)out | (uintptr_t)scratch) % 16 ||
+           ((long long)n / 16 + 1) * ((long long)m / 128 + 1) > 0x3fffffff;
 }
 
 }  // namespace jb
@@ -1003,7 +1004,7 @@ extern "C" int jb_linear_mx4_cta(int n, int m, int k, int rows, int *out)
 extern "C" int jb_linear_mx4(const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales, void *out,
                              int out_dt, int n, int m, int k, void *scratch, int w_early, cudaStream_t st)
 {
-    if (bad_product(a_codes, a_scales, w_codes, w_scales, scratch, out_dt, n, m, k))
+    if (bad_product(a_codes, a_scales, w_codes, w_scales, out, scratch, out_dt, n, m, k))
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;
@@ -1017,7 +1018,7 @@ extern "C" int jb_linear_mx4(const void *a_codes, const void *a_scales, const vo
 extern "C" int jb_linear_mx4_rows(const void *x, int dt, const void *w_codes, const void *w_scales, void *out, int out_dt, int n,
                                   int m, int k, void *scratch, int w_early, cudaStream_t st)
 {
-    if (bad_product(nullptr, nullptr, w_codes, w_scales, scratch, out_dt, n, m, k) || (dt != 0 && dt != 1))
+    if (bad_product(nullptr, nullptr, w_codes, w_scales, out, scratch, out_dt, n, m, k) || (dt != 0 && dt != 1))
         return JB_EINVAL;
     if (n == 0 || m == 0)
         return JB_OK;

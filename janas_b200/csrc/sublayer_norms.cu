@@ -276,7 +276,7 @@ using namespace jb;
 
 // y: a stack [Sy, n, dm]; g: a stack [Sg, n, g_ld] whose columns g_col0 .. g_col0 + dm - 1 are the gate, or null; biases,
 // weights and scale float32 [dm] or null (w1 null: no norm of the result; w2 null: no h).  out_kind: 0 float32, 1
-// bfloat16, 4 microscaled 4-bit floats (out the codes, out_scales the scales).
+// bfloat16, 4 microscaled 4-bit floats (out the codes, at an address that 16 divides, out_scales the scales).
 extern "C" int jb_norm_residual_norm(float *x, const float *y, int Sy, long long y_stride, const float *y_bias,
                                      const float *g, int Sg, long long g_stride, int g_ld, int g_col0, const float *g_bias,
                                      const float *w1, const float *b1, float eps1, const float *scale, float mult,
@@ -287,7 +287,7 @@ extern "C" int jb_norm_residual_norm(float *x, const float *y, int Sy, long long
         return JB_OK;
     if (n < 0 || dm < 1 || Sy < 1 || (g && (Sg < 1 || g_col0 < 0 || g_ld - g_col0 < dm)) || dm > jb_norm_residual_norm_most() ||
         (w2 && !out) || (out_kind != OUT_F32 && out_kind != OUT_BF16 && out_kind != OUT_MX4) ||
-        (w2 && out_kind == OUT_MX4 && !out_scales))
+        (w2 && out_kind == OUT_MX4 && (!out_scales || (uintptr_t)out % 16 != 0)))
         return JB_EINVAL;
     NormsArgs a{x, y, y_bias, g, g_bias, w1, b1, scale, w2, b2, Sy, Sg, g_ld, g_col0, rms, out_kind, dm,
                 (size_t)y_stride, (size_t)g_stride, eps1, mult, eps2, 1.0f / dm, out, (uint8_t *)out_scales};
