@@ -24,6 +24,7 @@
 // sublayer reads a weighted sum of them through its norm and all are mixed as its result joins:
 //     y = ls * sublayer(norm(sum_s in[s] X_s));   X_t <- sum_s mix[s, t] X_s + m out[t] y
 // for the mixer and then, where the layer has one, for the feed-forward, with weights of their own.
+#include "../csrc/kernels.h"
 #include "part.h"
 
 namespace jb {
@@ -115,6 +116,8 @@ public:
         if (bp.get("ffn_gate").is_string() && feed_forward) gate_name_[1] = bp.get("ffn_gate").as_string();
         if (bp.get("mixer_scale").is_string()) scale_name_[0] = bp.get("mixer_scale").as_string();
         if (bp.get("ffn_scale").is_string() && feed_forward) scale_name_[1] = bp.get("ffn_scale").as_string();
+        if (!(scale_name_[0].empty() && scale_name_[1].empty()) && hidden_ > jb_norm_residual_norm_most())
+            config_error(fmt("sandwich: a residual scale needs rows of at most %d values", jb_norm_residual_norm_most()));
         if (bp.get("gate_bias").is_string()) bias_suffix_ = bp.get("gate_bias").as_string();
         if (bp.get("fuse").is_bool()) fuse_ = bp.get("fuse").as_bool();
         const Json &ts = bp.get("token_side");

@@ -167,3 +167,26 @@ def test_residual_scales_step_by_step(kind, gates):
     # last one the model's), and with gates four gates
     assert count[False] > count[True] + 4
     assert rel_err(got[False], got[True]) <= 2 * 10 * 160 * 4 * torch.finfo(torch.float32).eps / 2
+
+
+def test_a_residual_scale_of_too_many_features():
+    """Longer rows than the kernel takes: refused when the model is opened, not in its first step."""
+    from dataclasses import replace
+    from janas_b200 import lib
+    from janas_b200.csrc import ops
+    from janas_b200.engine import Engine
+    spec = sandwich("swiglu", "layer", False, scales=True)
+    wide = ops.lib().jb_norm_residual_norm_most() + 4
+
+    def sized(part):
+        key = "size" if "size" in part.params else "hidden_size"
+        return replace(part, params={**part.params, key: wide})
+
+    layers = tuple(replace(l, mixer=sized(l.mixer), feed_forward=sized(l.feed_forward), mixer_norm=sized(l.mixer_norm),
+                           ffn_norm=sized(l.ffn_norm), post_mixer_norm=sized(l.post_mixer_norm),
+                           post_ffn_norm=sized(l.post_ffn_norm), block_params={**l.block_params, "hidden_size": wide})
+                   for l in spec.layers)
+    spec = replace(spec, hidden_size=wide, layers=layers, final_norm=sized(spec.final_norm))
+    with pytest.raises(lib.LLMError) as err:
+        Engine.from_spec(spec, seed=1, dtype="bfloat16", max_tokens=64)
+    assert "residual scale" in str(err.value)
