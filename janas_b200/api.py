@@ -31,7 +31,9 @@ class LLMParams:
     max_batch: int = 64         # most sequences that run together
     max_tokens: int = 0         # tokens the cache holds in all; 0: n_ctx
     device: str = "cuda:0"
-    weights: str = "stored"     # or "mx4": attention's and dense feed-forwards' matrices in 4 bits
+    # or "mx4": the matrices of gqa_attention and of the feed-forwards swiglu, polynorm and dense in 4 bits, and in each
+    # step what they are multiplied with; all else as stored
+    weights: str = "stored"
 
 
 def params_default() -> LLMParams:

@@ -103,7 +103,8 @@ def main(argv=None) -> int:
     ap.add_argument("--batch", type=int, default=1, help="sequences that run together")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--weights", default="stored", choices=["stored", "mx4"],
-                    help="mx4: the matrices of attention and dense feed-forwards in microscaled 4-bit floats")
+                    help="mx4: the matrices of gqa_attention and of the feed-forwards swiglu, polynorm and dense, and "
+                         "what they are multiplied with, in microscaled 4-bit floats; all else as stored")
     ap.add_argument("--stats", action="store_true")
     ap.add_argument("--chat", action="store_true", help="turns of token ids on standard input, "
                                                         "one a line; replies as lines of ids")

@@ -26,7 +26,8 @@ Engine::Engine(std::unique_ptr<Device> d, std::unique_ptr<DecoderModel> m, long 
     : dev(std::move(d)), model(std::move(m)), dtype(model->dtype) {
     if (!dev) fail(JB_LLM_EFAIL, "janas_b200 runs on a CUDA device only; there is no CPU path");
     if (model->mx4 && model->packed == 0)
-        fail(JB_LLM_EMODEL, "weights in 4 bits: no part of this model takes them (attention and dense feed-forwards do)");
+        fail(JB_LLM_EMODEL, "weights in 4 bits: no part of this model takes them (gqa_attention and the feed-forwards swiglu, "
+                            "polynorm and dense do)");
     if (jb_page() != PAGE)
         fail(JB_LLM_EFAIL, fmt("the kernels were built for pages of %d positions, the cache for %d",
                                jb_page(), PAGE));

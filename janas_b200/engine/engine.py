@@ -109,8 +109,9 @@ class Engine:
              max_seqs: Optional[int] = None, device: str = "cuda:0",
              n_ctx: Optional[int] = None, weights: str = "stored") -> "Engine":
         """Reads config.json, picks the model through the registry and loads the
-        folder's safetensors by tensor name.  weights "mx4": the matrices of attention and
-        dense feed-forwards in microscaled 4-bit floats (a bfloat16 model)."""
+        folder's safetensors by tensor name.  weights "mx4": the matrices of
+        gqa_attention and of the feed-forwards swiglu, polynorm and dense in microscaled 4-bit
+        floats, and step by step their products' inputs (a bfloat16 model)."""
         p = _params(dtype, max_tokens, max_seqs, device, n_ctx, weights)
         h = ctypes.c_void_p()
         lib.check(lib.lib().jb_llm_open(str(model_dir).encode(), ctypes.byref(p), ctypes.byref(h)))

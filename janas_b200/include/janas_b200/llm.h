@@ -46,9 +46,11 @@ extern "C" {
 #define JB_LLM_F32 1        /* the whole model in true 32-bit (no reduced-precision product) */
 
 #define JB_LLM_STORED 0     /* weights in their own type (bfloat16, or float32 where stored so) */
-#define JB_LLM_MX4 1        /* the matrices of attention and dense feed-forwards in microscaled 4-bit
-                               floats (blocks of 32 with a power of two each), brought to them when the
-                               model is opened; their products' inputs are brought to them step by step.
+#define JB_LLM_MX4 1        /* the matrices of gqa_attention and of the feed-forwards swiglu, polynorm
+                               and dense in microscaled 4-bit floats (blocks of 32 with a power of two
+                               each), brought to them when the model is opened; their products' inputs
+                               are brought to them step by step. Everything else (other attention, routed
+                               experts, recurrences, gates, norms, the embedding, the head) stays as stored.
                                JB_LLM_BF16 only; JB_LLM_EMODEL where no part of the model takes them. */
 
 typedef struct jb_llm jb_llm;                 /* an open model */

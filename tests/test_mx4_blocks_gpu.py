@@ -190,3 +190,15 @@ def test_a_residual_scale_of_too_many_features():
     with pytest.raises(lib.LLMError) as err:
         Engine.from_spec(spec, seed=1, dtype="bfloat16", max_tokens=64)
     assert "residual scale" in str(err.value)
+
+
+def test_the_refusal_names_the_parts():
+    """A design with attention of another kind and routed experts alone: none of its parts takes 4 bits, and the message
+    says which do."""
+    from janas_b200 import lib
+    from janas_b200.engine import Engine
+    from kefesun_models import CONFIGS
+    with pytest.raises(lib.LLMError) as err:
+        Engine.open_random(CONFIGS["KA"], weights="mx4")
+    assert err.value.code == lib.EMODEL
+    assert all(kind in str(err.value) for kind in ("gqa_attention", "swiglu", "polynorm", "dense"))
