@@ -17,7 +17,9 @@
 // the bytes take 14; with five groups and a quarter of the warps 42 from memory, with one group 37, though 8 rows then take
 // 3.5 instead of 4.2; with each block's next row prefetched into shared memory 36, into the L2 31).  Rows that whole 16-byte
 // loads do not fit, or longer ones, stay in shared memory.
-// How a row is shared out among the threads depends on its length alone, so its bits are the same in any batch.
+// How a row is shared out among the threads depends on its length and on whether whole 16-byte loads fit (every address, the
+// stacks' strides, the gate's width and first column), so its bits are the same in any batch that is laid out alike, as a
+// layer's are from step to step; rows that start elsewhere in memory may differ in their sums' order.
 #include "kernels.h"
 #include "mx4.cuh"
 
