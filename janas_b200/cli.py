@@ -5,7 +5,7 @@
                [--max N] [--eos ID] [--stop ID ...] [--batch B] [--dtype bfloat16|float32] [--weights stored|mx4]
                [--stats]
     janas-b200 <model-dir> --chat [the sampling options, --ctx, --max]     (turns on standard input)
-    janas-b200 <model-dir> --bench [--prompt N] [--gen N] [--rounds N] [--ctx N] [--batch B]
+    janas-b200 <model-dir> --bench [--prompt N] [--gen N] [--rounds N] [--ctx N] [--batch B] [--weights stored|mx4]
     janas-b200 --random-weights <config.json> --out <model-dir> [--seed S] [--store bfloat16|float32]
 
 ``--ctx --temp --top-k --top-p --min-p --seed --max`` mean what they mean for

@@ -13,7 +13,7 @@
 // an MMA may still read.
 //
 // Few rows may come as floats, in tiles of 16 or 32 rows: every CTA then brings its part of them to 4 bits itself (warps 2
-// to 9, a warp a row's two chunks at a time), which costs less than the launch of a kernel that does it once.
+// to 9, a warp a row's two chunks at a time), which saves the launch of a kernel that does it once (mx_rows_tile).
 //
 // Every wait on an mbarrier has a time limit, as in gemm_tc.cu; when it runs out, the error word says which.
 #include "kernels.h"
@@ -907,10 +907,17 @@ constexpr int MX_FEW = 128;         // rows up to which a product's tiles are si
 
 // Rows of a tile, 16 or 32, where the product's CTAs pack rows of floats themselves, or 0 where a kernel ahead does: up to 32
 // rows always, and up to 128 where a warp has at most 12 items (a row of a chunk) to pack, as each tile along m packs the
-// same rows again.  Tiles of 16 rows leave a warp the fewest; 32 where those would be over two an SM.  77 rows of floats x
-// 1,003 x 1,037 (8 parts, 2 items): 6.1 us on the device and 8.9 with the call; quantised by a call of its own before, 8.4
-// and 15.5; all rows in one tile of 128, 13.2 and 13.4.  128 x 2,560 x 1,037 (10 items): 10.5 and 11.0, by two calls 9.6
-// and 15.4.  77 x 2,560 x 4,096 (16 items, not taken): 12.4 and 13.4, by two calls 9.2 and 15.8.
+// same rows again.  Tiles of 16 rows leave a warp the fewest; 32 where those would be over two an SM.
+// The rule weighs a call from Python, in which a second launch and memory for the codes cost about 5 us: 77 rows of floats x
+// 1,003 x 1,037 8.9 us, quantised by a call of its own before 15.5; 128 x 2,560 x 1,037 10.0 and 15.4; 128 x 2,560 x 2,560,
+// with a kernel ahead, 14.3.  On the device alone, as a captured step pays for it, it holds for one token and for short k
+// only; with more rows, tiles along m or chunks of k the kernel ahead would be faster.  Rows of bfloat16, packed by the
+// product / by a kernel ahead, us (40 of the same in a graph, so with the weights in the L2):
+//     1 x 2,560 x 9,728    5.7 /  6.3     8 x 2,560 x 4,096   5.1 /  5.4     77 x 1,003 x 1,037   6.2 /  6.7
+//     1 x 19,456 x 2,560   6.5 /  5.9     8 x 19,456 x 2,560  8.5 /  5.9     40 x 6,144 x 2,560   8.2 /  6.5
+//     16 x 6,144 x 2,560   6.4 /  5.4    32 x 6,144 x 2,560  10.0 /  6.1     77 x 6,144 x 1,037   9.6 /  7.4
+//     16 x 19,456 x 2,560 10.9 /  6.0    32 x 19,456 x 2,560 21.0 /  6.4    128 x 2,560 x 1,037   9.5 /  7.5
+//     16 x 2,560 x 9,728   8.6 /  6.9    32 x 2,560 x 9,728  13.9 /  7.3     32 x 19,456 x 9,728 79.8 / 19.2
 static int mx_rows_tile(int n, int m, int k)
 {
     if (n <= 32)

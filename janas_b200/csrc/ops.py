@@ -1337,7 +1337,8 @@ class Mx4:
     ``scales``: uint8 [ceil(rows / 128), ceil(k / 256), 1024], for each 128 rows and 256 of k the
     exponents + 127 of the blocks of 32 values (255: the block stands for NaNs), block b of row r
     at 512 (b / 4 % 2) + 16 (r % 32) + 4 (r / 32 % 4) + b % 4 of chunk b / 8.  Bytes of rows past the
-    last one are not written and not used; those of blocks past a row's end are zero."""
+    last one are not written and not used.  Codes past k in a row's last block and the scales of blocks past its end
+    are zero, and must be in codes and scales that a caller brings: a product takes them in."""
 
     __slots__ = ("rows", "k", "settled", "_buf", "_codes", "_scales", "_at_codes", "_at_scales")
 
